@@ -8,6 +8,7 @@ CPU fallback: without the built library or without a CUDA device every call rais
 """
 import ctypes as C
 import enum
+import math
 import os
 
 import numpy as np
@@ -58,6 +59,14 @@ class VerifyArgs(C.Structure):
 class ScoreArgs(C.Structure):
     _fields_ = [("struct_bytes", _u32), ("rows", _i32), ("vocab", _i32), ("logits", _P), ("logits_stride", _i64),
                 ("top_n", _i32), ("logsumexp", _P), ("top1", _P), ("top_ids", _P), ("top_logprob", _P), ("status", _P)]
+
+
+class ConstrainArgs(C.Structure):
+    _fields_ = [("struct_bytes", _u32), ("sequences", _i32), ("rows_per_sequence", _i32), ("vocab", _i32), ("dtype", _i32),
+                ("biases", _i32), ("logits", _P), ("logits_stride", _i64), ("out", _P), ("out_stride", _i64),
+                ("repetition", _f32), ("presence", _f32), ("frequency", _f32), ("fill", _f32), ("penalties", _P),
+                ("history", _P), ("history_stride", _i64), ("history_len", _P), ("draft_ids", _P), ("bias_ids", _P),
+                ("bias_values", _P), ("mask", _P), ("mask_stride", _i64), ("status", _P)]
 
 
 class ProbArgs(C.Structure):
@@ -111,6 +120,7 @@ def lib():
         L.ds41_b200_sample_probabilities.argtypes = [_P, C.c_int, C.c_int, _i64, _P, _P, C.c_uint32, C.c_uint32, _P, _P, _P]
         L.ds41_b200_verify_probabilities.argtypes = [_P, _P, _P, C.c_int, C.c_int, C.c_int, C.c_int, _P, _P, _P, _P, _P]
         L.ds41_b200_probabilities.argtypes = [C.POINTER(ProbArgs), _P]
+        L.ds41_b200_constrain_logits.argtypes = [C.POINTER(ConstrainArgs), _P]
         _lib = L
     return _lib
 
@@ -148,6 +158,25 @@ def _dev(t, dtype, name):
         return None
     if not t.is_cuda or t.dtype != dtype or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous CUDA tensor of {dtype}")
+    return t
+
+
+_ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # DS41_B200_F32, _BF16, _F16
+
+
+def _rows(t, dtypes, name, device, shape):
+    """The row stride of a 2-D tensor of that shape (None: any extent) with unit inner stride on `device`."""
+    if not t.is_cuda or t.device != device or t.dtype not in dtypes or t.dim() != 2 or \
+            any(n is not None and n != m for n, m in zip(shape, t.shape)) or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be a tensor of {' or '.join(map(str, dtypes))} on {device} of {shape} rows and columns, "
+                         f"columns next to each other")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _flat(t, dtype, name, device, count):
+    """`t` itself, checked: contiguous, on `device`, `count` elements."""
+    if not t.is_cuda or t.device != device or t.dtype != dtype or t.numel() != count or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor of {count} {dtype} on {device}")
     return t
 
 
@@ -233,6 +262,67 @@ def sample_logits(logits, temperature, top_p, seeds, steps, slot=0, purpose=Purp
     a.row_extremes = row_extremes.data_ptr() if row_extremes is not None else None
     _launch(logits.device, "ds41_b200_sample_logits", lib().ds41_b200_sample_logits, C.byref(a))
     return tokens, status
+
+
+def constrain_logits(logits, history=None, history_len=None, repetition=1.0, presence=0.0, frequency=0.0, penalties=None,
+                     draft_ids=None, rows_per_sequence=1, bias_ids=None, bias_values=None, mask=None, fill=None, out=None,
+                     status=None):
+    """Penalties, biases and the grammar bitmask applied to rows of logits, for the calls that take plain rows: the verifier,
+    the score report, the probability rows, the sampler's larger batches, the distillation.
+
+    logits fp32, bf16 or fp16 [rows, vocab] (columns next to each other; rows any stride).  Row s * rows_per_sequence + j is
+    position j of sequence s: it counts history[s, :history_len[s]] (int32 [sequences, n], ids outside the vocabulary are
+    padding) and the first j of draft_ids[s] (int32 [sequences, rows_per_sequence - 1]).
+    repetition / presence / frequency: for every sequence, or penalties fp32 [sequences, 3] with each sequence's own.
+    bias_ids int32 / bias_values fp32 [sequences, n]: added to those ids' logits (ids outside the vocabulary are padding).
+    mask int32 [rows, >= ceil(vocab / 32)]: allowed-token bits; other ids get `fill` (None: the lowest finite value).
+    out: None allocates; logits itself works in place.  Returns (out, status int32 [rows]); see ds41_b200.h for the rule and
+    the status words."""
+    if logits.dim() != 2 or not logits.is_cuda or logits.dtype not in _ROW_TYPES:
+        raise ValueError("logits must be a CUDA fp32, bf16 or fp16 [rows, vocab] tensor")
+    rows, vocab = logits.shape
+    dev = logits.device
+    logits_stride = _rows(logits, (logits.dtype,), "logits", dev, (rows, vocab))
+    if rows_per_sequence < 1 or rows % rows_per_sequence:
+        raise ValueError("rows must be a multiple of rows_per_sequence")
+    sequences = rows // rows_per_sequence
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
+    out_stride = _rows(out, (logits.dtype,), "out", dev, (rows, vocab))
+    if status is None:
+        status = torch.empty(rows, dtype=torch.int32, device=dev)
+    _flat(status, torch.int32, "status", dev, rows)
+    if history is None and history_len is not None:
+        raise ValueError("history_len without history")
+    if (bias_ids is None) != (bias_values is None):
+        raise ValueError("bias_ids and bias_values come together")
+    history_stride = biases = mask_stride = 0
+    if history is not None:
+        history_stride = _rows(_flat(history, torch.int32, "history", dev, history.numel()), (torch.int32,), "history", dev,
+                               (sequences, None))
+        if history_len is not None:
+            _flat(history_len, torch.int32, "history_len", dev, sequences)
+    if penalties is not None:
+        _flat(penalties, torch.float32, "penalties", dev, 3 * sequences)
+    if draft_ids is not None:
+        _flat(draft_ids, torch.int32, "draft_ids", dev, sequences * (rows_per_sequence - 1))
+    if bias_ids is not None:
+        biases = bias_ids.shape[-1]
+        _flat(bias_ids, torch.int32, "bias_ids", dev, sequences * biases)
+        _flat(bias_values, torch.float32, "bias_values", dev, sequences * biases)
+    if mask is not None:
+        mask_stride = _rows(mask, (torch.int32,), "mask", dev, (rows, None))
+    lowest = torch.finfo(logits.dtype).min
+    if fill is None:
+        fill = lowest
+    elif math.isfinite(fill):    # (within the type's range, and so within the argument's)
+        fill = min(max(fill, lowest), -lowest)
+    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+    a = ConstrainArgs(C.sizeof(ConstrainArgs), sequences, rows_per_sequence, vocab, _ROW_TYPES[logits.dtype], biases, logits.data_ptr(),
+                      logits_stride, out.data_ptr(), out_stride, repetition, presence, frequency, fill, ptr(penalties), ptr(history), history_stride,
+                      ptr(history_len), ptr(draft_ids), ptr(bias_ids), ptr(bias_values), ptr(mask), mask_stride, status.data_ptr())
+    _launch(dev, "ds41_b200_constrain_logits", lib().ds41_b200_constrain_logits, C.byref(a))
+    return out, status
 
 
 def verify_scratch_bytes(sequences, drafts, vocab=MAX_VOCAB):

@@ -360,6 +360,54 @@ int ds41_b200_score_logits(const ds41_b200_score_args *args, cudaStream_t stream
 int ds41_b200_logits_sha256(const float *logits, int rows, int vocab, int64_t logits_stride, uint8_t *digests,
                             cudaStream_t stream);
 
+/* ---- constraints on logits rows: penalties, biases and the grammar bitmask as an operator of its own ------------------------
+ * What ds41_b200_sample_logits applies inside one of its paths, for every call that takes plain rows (the verifier, the score
+ * report, the probability rows, the larger batches of the sampler, the distillation below), with one set of penalties per
+ * sequence, biases, and the rows of a speculative transaction.  No counterpart in the reference.
+ * Row r = s * rows_per_sequence + j belongs to sequence s.  count[id] = occurrences of id in the first history_len[s] ids of the
+ * sequence's history and in the first j of its draft ids (row j verifies what follows j drafts).  In FP32, every operation
+ * rounded separately: y = x; if count > 0: y = x > 0 ? x / repetition : x * repetition, then y -= presence + frequency *
+ * float(count) (the sampler's rule: the same bits); if the bias list names the id: y += the sum of its entries in the list's
+ * order; rounded once to the rows' type.  Ids whose mask bit is 0 get `fill` instead, whatever their logit holds.  A finite fill
+ * is held within the type's range: -FLT_MAX gives the lowest value of any type, which the calls behind take like any logit;
+ * -INFINITY suits the distillation and host code, while the sampler and its like reject a row that holds it.
+ * status[r]: 0, or the first that holds of
+ *   DS41_B200_ROW_PARAMETER (repetition not positive, or a penalty not finite), DS41_B200_ROW_HISTORY (history_len negative, above
+ *   history_stride, or with the drafts above DS41_B200_CONSTRAIN_MAX_HISTORY), DS41_B200_ROW_EMPTY (the mask allows no id): the
+ *   row is written as NaN, so that no call behind can take it for a row of logits;
+ *   DS41_B200_ROW_NONFINITE (an allowed logit is NaN or infinite), DS41_B200_ROW_PENALTY_OVERFLOW (an allowed result is not finite
+ *   in the rows' type): the row holds what the rule gives, so that it is rejected too. */
+#define DS41_B200_F32 0
+#define DS41_B200_BF16 1
+#define DS41_B200_F16 2
+#define DS41_B200_F64 3
+#define DS41_B200_ROW_PARAMETER (-11)
+#define DS41_B200_CONSTRAIN_MAX_HISTORY 65534 /* one counter value marks the ids of the bias list */
+#define DS41_B200_CONSTRAIN_MAX_BIASES 1024
+typedef struct ds41_b200_constrain_args {
+  uint32_t struct_bytes;
+  int32_t sequences, rows_per_sequence, vocab; /* 1 <= vocab <= DS41_B200_MAX_VOCAB */
+  int32_t dtype;               /* of logits and out: DS41_B200_F32, _BF16 or _F16 */
+  int32_t biases;              /* entries of a sequence's bias list, 0..DS41_B200_CONSTRAIN_MAX_BIASES */
+  const void *logits;          /* [rows, logits_stride] */
+  int64_t logits_stride;       /* elements: >= vocab, or 0 to give every row the same logits */
+  void *out;                   /* [rows, out_stride]; may be logits with the same stride (in place), no other overlap */
+  int64_t out_stride;
+  float repetition, presence, frequency; /* for every sequence, where penalties is NULL; 1,0,0 = off */
+  float fill;
+  const float *penalties;      /* [sequences, 3] repetition, presence, frequency of each sequence, or NULL */
+  const int32_t *history;      /* [sequences, history_stride] token ids or NULL; ids outside [0,vocab) are padding */
+  int64_t history_stride;
+  const int32_t *history_len;  /* [sequences] or NULL = history_stride for every sequence */
+  const int32_t *draft_ids;    /* [sequences, rows_per_sequence - 1] or NULL */
+  const int32_t *bias_ids;     /* [sequences, biases]; ids outside [0,vocab) are padding */
+  const float *bias_values;    /* [sequences, biases] */
+  const uint32_t *mask;        /* [rows, mask_stride] allowed-token bits (id/32, id%32) or NULL */
+  int64_t mask_stride;
+  int32_t *status;             /* [rows] out; may be NULL */
+} ds41_b200_constrain_args;
+int ds41_b200_constrain_logits(const ds41_b200_constrain_args *args, cudaStream_t stream);
+
 /* Measurement hook (not thread-safe, off by default): with it on, the next ds41_b200_sample_logits call that takes the
  * batch path records CUDA events on its stream between its kernels; ds41_b200_profile_read waits for the last one and
  * returns the milliseconds of each interval, in launch order: statistics, histogram, window, masses, resolve, cluster
