@@ -14,6 +14,12 @@ template <> struct RowType<float> {
   static constexpr float kMax = 3.402823466e+38f;
   static __device__ __forceinline__ float load(float v) { return v; }
   static __device__ __forceinline__ float store(float v) { return v; }
+  // 0, or NaN once any value that went through was NaN or infinite
+  using Finite = float;
+  static __device__ __forceinline__ Finite check(const uint4 &q, Finite f) {
+    return fmaf(__uint_as_float(q.x), 0.f, fmaf(__uint_as_float(q.y), 0.f, fmaf(__uint_as_float(q.z), 0.f, fmaf(__uint_as_float(q.w), 0.f, f))));
+  }
+  static __device__ __forceinline__ bool all_finite(Finite f) { return f == 0.f; }
   static __device__ __forceinline__ void unpack(const uint4 &q, float (&x)[4]) {
     x[0] = __uint_as_float(q.x); x[1] = __uint_as_float(q.y); x[2] = __uint_as_float(q.z); x[3] = __uint_as_float(q.w);
   }
@@ -26,6 +32,18 @@ template <> struct RowType<__nv_bfloat16> {
   static constexpr float kMax = 3.38953139e+38f;   // 0x7f7f
   static __device__ __forceinline__ float load(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ __nv_bfloat16 store(float v) { return __float2bfloat16_rn(v); }
+  using Finite = __nv_bfloat162;
+  static __device__ __forceinline__ Finite check(const uint4 &q, Finite f) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      Finite v;
+      *reinterpret_cast<uint32_t *>(&v) = w[k];
+      f = __hfma2(v, __float2bfloat162_rn(0.f), f);
+    }
+    return f;
+  }
+  static __device__ __forceinline__ bool all_finite(Finite f) { return __low2float(f) == 0.f && __high2float(f) == 0.f; }
   static __device__ __forceinline__ void unpack(const uint4 &q, float (&x)[8]) {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -43,6 +61,18 @@ template <> struct RowType<__half> {
   static constexpr float kMax = 65504.f;
   static __device__ __forceinline__ float load(__half v) { return __half2float(v); }
   static __device__ __forceinline__ __half store(float v) { return __float2half_rn(v); }
+  using Finite = __half2;
+  static __device__ __forceinline__ Finite check(const uint4 &q, Finite f) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      Finite v;
+      *reinterpret_cast<uint32_t *>(&v) = w[k];
+      f = __hfma2(v, __float2half2_rn(0.f), f);
+    }
+    return f;
+  }
+  static __device__ __forceinline__ bool all_finite(Finite f) { return __low2float(f) == 0.f && __high2float(f) == 0.f; }
   static __device__ __forceinline__ void unpack(const uint4 &q, float (&x)[8]) {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll

@@ -373,8 +373,8 @@ int ds41_b200_logits_sha256(const float *logits, int rows, int vocab, int64_t lo
  * -INFINITY suits the distillation and host code, while the sampler and its like reject a row that holds it.
  * status[r]: 0, or the first that holds of
  *   DS41_B200_ROW_PARAMETER (repetition not positive, or a penalty not finite), DS41_B200_ROW_HISTORY (history_len negative, above
- *   history_stride, or with the drafts above DS41_B200_CONSTRAIN_MAX_HISTORY), DS41_B200_ROW_EMPTY (the mask allows no id): the
- *   row is written as NaN, so that no call behind can take it for a row of logits;
+ *   history_stride, or with the drafts above DS41_B200_MAX_HISTORY), DS41_B200_ROW_EMPTY (the mask allows no id): the row is
+ *   written as NaN, so that no call behind can take it for a row of logits;
  *   DS41_B200_ROW_NONFINITE (an allowed logit is NaN or infinite), DS41_B200_ROW_PENALTY_OVERFLOW (an allowed result is not finite
  *   in the rows' type): the row holds what the rule gives, so that it is rejected too. */
 #define DS41_B200_F32 0
@@ -382,7 +382,6 @@ int ds41_b200_logits_sha256(const float *logits, int rows, int vocab, int64_t lo
 #define DS41_B200_F16 2
 #define DS41_B200_F64 3
 #define DS41_B200_ROW_PARAMETER (-11)
-#define DS41_B200_CONSTRAIN_MAX_HISTORY 65534 /* one counter value marks the ids of the bias list */
 #define DS41_B200_CONSTRAIN_MAX_BIASES 1024
 typedef struct ds41_b200_constrain_args {
   uint32_t struct_bytes;

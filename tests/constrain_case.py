@@ -26,7 +26,7 @@ def expected(x, dtype, history=None, lens=None, penalties=None, drafts=None, per
                 out[r], status[r] = np.nan, -11
                 continue
             n = 0 if history is None else history.shape[1] if lens is None else int(lens[s])
-            if n < 0 or (history is not None and n > history.shape[1]) or n + (j if drafts is not None else 0) > 65534:
+            if n < 0 or (history is not None and n > history.shape[1]) or n + (j if drafts is not None else 0) > 65535:
                 out[r], status[r] = np.nan, -7
                 continue
             allowed = bits_of(mask[r:r + 1], vocab)[0] if mask is not None else np.ones(vocab, bool)

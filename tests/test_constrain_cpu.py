@@ -39,7 +39,7 @@ def good(pkg, **changes):
     ({"out": (1 << 20) + 4000}, "overlaps"), ({"out": 1 << 20, "out_stride": 1001}, "overlaps"), ({"out": 1 << 20, "logits_stride": 0}, "overlaps"),
     ({"out": (1 << 20) - 23996}, "overlaps"), ({"out": (1 << 20) + 4 * 900, "logits_stride": 2000, "out_stride": 2000}, "overlaps"),
     ({"repetition": 0.0}, "penalties"), ({"repetition": float("nan")}, "penalties"), ({"presence": float("inf")}, "penalties"),
-    ({"history": 1 << 12, "history_stride": -1}, "history"), ({"history": 1 << 12, "history_stride": 65535}, "history"),
+    ({"history": 1 << 12, "history_stride": -1}, "history"), ({"history": 1 << 12, "history_stride": 65536}, "history"),
     ({"biases": -1}, "biases"), ({"biases": 1025, "bias_ids": 1, "bias_values": 1}, "biases"), ({"biases": 1, "bias_ids": 1}, "no list"),
     ({"mask": 1 << 12, "mask_stride": 31}, "mask stride"), ({"fill": float("nan")}, "NaN")])
 def test_arguments_are_refused_before_any_launch(pkg, changes, message):

@@ -48,7 +48,7 @@ def test_rows_of_every_size_type_and_alignment(pkg, dtype, vocab, lead, gap):
 
 
 @pytest.mark.parametrize("sequences,per,history,biases,share", [
-    (1, 1, 1, 0, None), (1, 1, 0, 0, 0.5), (1, 1, 65534, 1024, None), (2, 6, 65529, 3, 0.01), (2, 6, 65530, 0, None), (5, 1, 0, 1, None), (160, 1, 100, 0, 0.9),
+    (1, 1, 1, 0, None), (1, 1, 0, 0, 0.5), (1, 1, 65535, 1024, None), (2, 6, 65530, 3, 0.01), (2, 6, 65531, 0, None), (5, 1, 0, 1, None), (160, 1, 100, 0, 0.9),
     (40, 4, 5000, 300, 0.02), (3, 1, 4099, 17, 0.0005)])
 @pytest.mark.parametrize("dtype,vocab", [("fp32", 129280), ("bf16", 40001)])
 def test_lengths_and_lists(pkg, sequences, per, history, biases, share, dtype, vocab):
@@ -57,9 +57,9 @@ def test_lengths_and_lists(pkg, sequences, per, history, biases, share, dtype, v
 
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_one_id_through_the_whole_history_and_the_whole_list(pkg, dtype):
-    """The largest count (65534 occurrences), and every entry of the longest list for the same id."""
-    c = case(4, 2, 3000, TYPES[dtype], history=65534, biases=1024)
-    c["lens"][:] = 65534
+    """The largest count (65535 occurrences), and every entry of the longest list for the same id."""
+    c = case(4, 2, 3000, TYPES[dtype], history=65535, biases=1024)
+    c["lens"][:] = 65535
     c["history"][0] = 2999
     c["penalties"][:, 2] = 1e-4
     c["bias_ids"][0] = 2999
