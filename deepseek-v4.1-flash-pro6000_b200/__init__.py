@@ -69,6 +69,14 @@ class ConstrainArgs(C.Structure):
                 ("bias_values", _P), ("mask", _P), ("mask_stride", _i64), ("status", _P)]
 
 
+class DistillArgs(C.Structure):
+    _fields_ = [("struct_bytes", _u32), ("rows", _i32), ("vocab", _i32), ("dtype", _i32), ("teacher_dtype", _i32), ("top", _i32),
+                ("tail", _i32), ("reserved", _i32), ("logits", _P), ("logits_stride", _i64), ("teacher_ids", _P),
+                ("ids_stride", _i64), ("teacher_values", _P), ("values_stride", _i64), ("temperature", _f64), ("mask", _P),
+                ("mask_stride", _i64), ("row_scale", _P), ("loss", _P), ("stats", _P), ("grad", _P), ("grad_stride", _i64),
+                ("status", _P)]
+
+
 class ProbArgs(C.Structure):
     _fields_ = [("struct_bytes", C.c_uint32), ("rows", C.c_int32), ("vocab", C.c_int32), ("logits", C.c_void_p),
                 ("logits_stride", C.c_int64), ("temperature", C.c_double), ("top_p", C.c_double),
@@ -121,6 +129,8 @@ def lib():
         L.ds41_b200_verify_probabilities.argtypes = [_P, _P, _P, C.c_int, C.c_int, C.c_int, C.c_int, _P, _P, _P, _P, _P]
         L.ds41_b200_probabilities.argtypes = [C.POINTER(ProbArgs), _P]
         L.ds41_b200_constrain_logits.argtypes = [C.POINTER(ConstrainArgs), _P]
+        for name in ("loss", "grad", "loss_grad"):
+            getattr(L, "ds41_b200_distill_" + name).argtypes = [C.POINTER(DistillArgs), _P]
         _lib = L
     return _lib
 
@@ -497,6 +507,80 @@ def score_logits(logits, top_n=0):
                   top1.data_ptr(), ids.data_ptr() if top_n else None, lp.data_ptr() if top_n else None, status.data_ptr())
     _launch(dev, "ds41_b200_score_logits", lib().ds41_b200_score_logits, C.byref(a))
     return lse, top1, ids, lp, status
+
+
+def _distill_args(logits, teacher_ids, teacher_values, temperature, tail, mask, row_scale):
+    """What the three calls share, checked."""
+    if logits.dim() != 2 or not logits.is_cuda or logits.dtype not in _ROW_TYPES:
+        raise ValueError("logits must be a CUDA fp32, bf16 or fp16 [rows, vocab] tensor")
+    rows, vocab = logits.shape
+    dev = logits.device
+    a = DistillArgs()
+    a.struct_bytes = C.sizeof(DistillArgs)
+    a.rows, a.vocab, a.dtype, a.tail = rows, vocab, _ROW_TYPES[logits.dtype], 1 if tail else 0
+    a.logits, a.logits_stride = logits.data_ptr(), _rows(logits, (logits.dtype,), "logits", dev, (rows, vocab))
+    a.ids_stride = _rows(teacher_ids, (torch.int32,), "teacher_ids", dev, (rows, None))
+    a.top = teacher_ids.shape[1]
+    a.values_stride = _rows(teacher_values, (torch.float32, torch.float64), "teacher_values", dev, (rows, a.top))
+    a.teacher_ids, a.teacher_values = teacher_ids.data_ptr(), teacher_values.data_ptr()
+    a.teacher_dtype = 3 if teacher_values.dtype == torch.float64 else 0
+    a.temperature = temperature
+    if mask is not None:
+        a.mask, a.mask_stride = mask.data_ptr(), _rows(mask, (torch.int32,), "mask", dev, (rows, None))
+    if row_scale is not None:
+        a.row_scale = _flat(row_scale, torch.float32, "row_scale", dev, rows).data_ptr()
+    return a
+
+
+def _distill_grad_buffer(a, logits, out):
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    a.grad, a.grad_stride = out.data_ptr(), _rows(out, (logits.dtype,), "out", logits.device, logits.shape)
+    return out
+
+
+def distill_loss(logits, teacher_ids, teacher_values, temperature=1.0, tail=False, mask=None):
+    """Distillation loss of a draft head's logits (fp32, bf16 or fp16 [rows, vocab]) against the target's top logits: teacher_ids
+    int32 and teacher_values fp32 or fp64 [rows, n], n <= 256, as score_logits(top_n=n) returns them (top_ids, top_logprob) or as
+    they were stored; ids outside the vocabulary are padding.  tail=False: the teacher is softmax(values / temperature) over its
+    list; tail=True (temperature 1): the values are log-probabilities, and what they leave belongs to the ids outside the list.
+    mask int32 [rows, >= ceil(vocab / 32)]: allowed-token bits, as in sample_logits; a logit of -inf is not allowed either.
+    Returns (loss fp32 [rows], stats fp32 [rows, 4] for distill_grad, status int32 [rows]); see ds41_b200.h for the formulas."""
+    a = _distill_args(logits, teacher_ids, teacher_values, temperature, tail, mask, None)
+    dev = logits.device
+    loss = torch.empty(a.rows, dtype=torch.float32, device=dev)
+    stats = torch.empty((a.rows, 4), dtype=torch.float32, device=dev)
+    status = torch.empty(a.rows, dtype=torch.int32, device=dev)
+    a.loss, a.stats, a.status = loss.data_ptr(), stats.data_ptr(), status.data_ptr()
+    _launch(dev, "ds41_b200_distill_loss", lib().ds41_b200_distill_loss, C.byref(a))
+    return loss, stats, status
+
+
+def distill_grad(logits, teacher_ids, teacher_values, stats, row_scale=None, temperature=1.0, tail=False, mask=None, out=None):
+    """The gradient of row_scale[r] * loss[r] by logits (the upstream gradient of each row's loss; None = 1; rows with 0 are not
+    read) from distill_loss's stats and the same other arguments.  out: None allocates; logits itself works in place.
+    Returns the gradient in the logits' type."""
+    a = _distill_args(logits, teacher_ids, teacher_values, temperature, tail, mask, row_scale)
+    if stats.dim() != 2 or stats.shape[1] != 4:
+        raise ValueError("stats must be [rows, 4]")
+    a.stats = _flat(stats, torch.float32, "stats", logits.device, 4 * a.rows).data_ptr()
+    out = _distill_grad_buffer(a, logits, out)
+    _launch(logits.device, "ds41_b200_distill_grad", lib().ds41_b200_distill_grad, C.byref(a))
+    return out
+
+
+def distill_loss_grad(logits, teacher_ids, teacher_values, row_scale=None, temperature=1.0, tail=False, mask=None, out=None):
+    """Loss and gradient in one call that reads the logits once: distill_loss and distill_grad with row_scale known beforehand
+    (rows with 0 are not read: loss 0, gradient 0).  out: None allocates; logits itself works in place.
+    Returns (loss fp32 [rows], gradient in the logits' type, status int32 [rows])."""
+    a = _distill_args(logits, teacher_ids, teacher_values, temperature, tail, mask, row_scale)
+    dev = logits.device
+    loss = torch.empty(a.rows, dtype=torch.float32, device=dev)
+    status = torch.empty(a.rows, dtype=torch.int32, device=dev)
+    a.loss, a.status = loss.data_ptr(), status.data_ptr()
+    out = _distill_grad_buffer(a, logits, out)
+    _launch(dev, "ds41_b200_distill_loss_grad", lib().ds41_b200_distill_loss_grad, C.byref(a))
+    return loss, out, status
 
 
 def probabilities(logits, temperature, top_p):

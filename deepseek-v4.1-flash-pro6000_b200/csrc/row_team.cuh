@@ -1,6 +1,6 @@
 // The CTAs of one cluster that share a logits row, a slice of its ids each ("team"): rank, barrier, and reads of another
 // CTA's shared memory.  Such a read lies behind a team_barrier(), without which that CTA need not have started or written, and in
-// front of another one, without which it may have left.
+// front of another one (or of a team_arrive() whose team_wait() ends the kernel), without which it may have left.
 #pragma once
 #include <stdint.h>
 
@@ -20,6 +20,15 @@ __device__ __forceinline__ uint32_t team_size() {
 __device__ __forceinline__ void team_barrier() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The barrier in two halves, with work in between that the others need not wait for.
+__device__ __forceinline__ void team_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void team_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ uint32_t team_address(const void *p, uint32_t rank) {
   uint32_t a;

@@ -407,6 +407,59 @@ typedef struct ds41_b200_constrain_args {
 } ds41_b200_constrain_args;
 int ds41_b200_constrain_logits(const ds41_b200_constrain_args *args, cudaStream_t stream);
 
+/* ---- distillation of a draft head from the target's top logits: loss and gradient of logits rows ------------------------------
+ * The teacher's row is a list of ids and values, as ds41_b200_score_logits leaves them (top_ids, top_logprob) or as they were
+ * stored; the student's is a row of logits.  No counterpart in the reference (it does not train).
+ * With T = temperature, u_i = z_i / T over the ids that are allowed (mask bit set, z_i > -inf), q = softmax(u):
+ *   entries: those whose id is in [0, vocab) and allowed count; entries of the same id add up; any other is padding
+ *   tail = 0: p_j = exp(value_j / T) over the list, normalised to 1
+ *   tail = 1 (T = 1): p_j = exp(value_j), values being log-probabilities over the teacher's whole row; the ids outside the list have
+ *             together rest = max(0, 1 - sum of the list) (nothing where every allowed id is listed); all normalised to 1
+ *   loss = T^2 (sum_j p_j (ln p_j - ln q_j) + rest (ln rest - ln q_rest)), q_rest = the student's share of the ids outside the list
+ *   grad_i = row_scale * d loss / d z_i = row_scale * T (q_i - p_i) for listed ids, row_scale * T (q_rest - rest) q_i / q_rest for
+ *            the others, 0 for ids that are not allowed
+ * Sums, maxima and everything per row are held in FP32 (the student's sum) or FP64 (the list, the logarithms); a gradient is
+ * rounded once to the rows' type.
+ * stats [rows, 4]: the largest allowed logit, ln sum exp((z - largest) / T), and the same two over the allowed ids outside the list
+ * (-inf where there are none): what _grad needs of _loss.  row_scale [rows] (NULL = 1): the gradient of the caller's loss by each row's;
+ * a row whose scale is 0 (padding) is not read: gradient 0, loss, stats and status 0.
+ * status[r]: 0, or the first that holds of
+ *   DS41_B200_ROW_NONFINITE (the value of an entry in the vocabulary is NaN or +inf, or an allowed logit that an entry names is),
+ *   DS41_B200_ROW_NOT_NORMALIZED (tail: the list's probabilities add up to more than 1.01),
+ *   DS41_B200_ROW_EMPTY (no entry counts, or all that do have probability 0): loss and gradient 0, stats NaN,
+ *   DS41_B200_ROW_NONFINITE (any other allowed logit is NaN or +inf);
+ * loss, stats and gradient of the other negative words are NaN.
+ * _loss writes loss, status and, where not NULL, stats; _grad reads stats and writes grad; _loss_grad reads the logits once and writes
+ * loss, grad, status and, where not NULL, stats.  grad may be logits with the same stride (in place), no other overlap. */
+#define DS41_B200_DISTILL_MAX_TOP 256
+typedef struct ds41_b200_distill_args {
+  uint32_t struct_bytes;
+  int32_t rows, vocab;         /* 1 <= vocab <= DS41_B200_MAX_VOCAB */
+  int32_t dtype;               /* of logits and grad: DS41_B200_F32, _BF16 or _F16 */
+  int32_t teacher_dtype;       /* of teacher_values: DS41_B200_F32 or _F64 */
+  int32_t top;                 /* entries of a row, 1..DS41_B200_DISTILL_MAX_TOP */
+  int32_t tail;                /* 0 or 1 */
+  int32_t reserved;            /* 0 */
+  const void *logits;          /* [rows, logits_stride] */
+  int64_t logits_stride;       /* elements, >= vocab */
+  const int32_t *teacher_ids;  /* [rows, ids_stride] */
+  int64_t ids_stride;
+  const void *teacher_values;  /* [rows, values_stride] */
+  int64_t values_stride;
+  double temperature;          /* finite, 1e-3..1e3 */
+  const uint32_t *mask;        /* [rows, mask_stride] allowed-token bits (id/32, id%32) or NULL */
+  int64_t mask_stride;
+  const float *row_scale;      /* [rows] or NULL; of the gradient's calls */
+  float *loss;                 /* [rows] out */
+  float *stats;                /* [rows, 4] out; in for _grad; 16-byte aligned */
+  void *grad;                  /* [rows, grad_stride] out */
+  int64_t grad_stride;
+  int32_t *status;             /* [rows] out */
+} ds41_b200_distill_args;
+int ds41_b200_distill_loss(const ds41_b200_distill_args *args, cudaStream_t stream);
+int ds41_b200_distill_grad(const ds41_b200_distill_args *args, cudaStream_t stream);
+int ds41_b200_distill_loss_grad(const ds41_b200_distill_args *args, cudaStream_t stream);
+
 /* Measurement hook (not thread-safe, off by default): with it on, the next ds41_b200_sample_logits call that takes the
  * batch path records CUDA events on its stream between its kernels; ds41_b200_profile_read waits for the last one and
  * returns the milliseconds of each interval, in launch order: statistics, histogram, window, masses, resolve, cluster

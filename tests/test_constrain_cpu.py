@@ -10,7 +10,7 @@ import torch
 
 import __graft_entry__ as entry
 from constrain_case import case, expected
-from test_kernel_rules_cpu import CSRC, enclosing, kernels, source, without_lambdas
+from test_kernel_rules_cpu import CSRC, braced, enclosing, kernels, source, without_lambdas
 
 
 @pytest.fixture(scope="module")
@@ -72,8 +72,8 @@ TEAM_READ = re.compile(r"\bteam_read\(|\bteam_address\(")
 
 
 def test_team_kernels_read_between_barriers():
-    """Another CTA's shared memory is read behind a barrier of the whole team and in front of one, both passed by every thread of every
-    CTA that has not left before the first of them."""
+    """Another CTA's shared memory is read behind a barrier of the whole team and in front of one (or of the first half of one whose second
+    half ends the kernel), which every thread of every CTA passes that has not left before the first of them."""
     seen = set()
     for name, kernel, _, body in kernels():
         text = without_lambdas(body)
@@ -81,11 +81,19 @@ def test_team_kernels_read_between_barriers():
             assert not TEAM_READ.search(body), (name, kernel)
             continue
         seen.add(kernel)
-        barriers = [m.start() for m in re.finditer(r"\bteam_barrier\(\);", text) if not enclosing(text, m.start())]
-        assert len(barriers) >= 2 and len(re.findall(r"\bteam_barrier\(", text)) == len(barriers), kernel
+        variant = "if constexpr (kTeam) {"        # (a kernel may have a variant without teams)
+        if variant in text:
+            part = braced(text, text.index(variant))
+            assert not TEAM_READ.search(text.replace(part, "")) and "team_barrier" not in text.replace(part, ""), kernel
+            text = part
+        barriers = [m.start() for m in re.finditer(r"\bteam_(?:barrier|arrive|wait)\(\);", text)]
+        assert not any(enclosing(text, b) for b in barriers), kernel
+        kinds = re.findall(r"\bteam_(barrier|arrive|wait)\(", text)
+        assert kinds in (["barrier", "barrier"], ["barrier", "arrive", "wait"]), (kernel, kinds)
         accesses = [m.start() for m in TEAM_READ.finditer(text)]
-        assert accesses and barriers[0] < accesses[0] and accesses[-1] < barriers[-1], kernel
-        assert "return;" not in text[barriers[0]:barriers[-1]], kernel
-    assert "constrain_kernel" in seen
+        assert accesses and barriers[0] < accesses[0] and accesses[-1] < barriers[1], kernel
+        assert "return;" not in text[barriers[0]:], kernel
+        assert text[barriers[-1]:].strip() in ("team_barrier();", "team_wait();"), kernel
+    assert seen == {"constrain_kernel", "distill_kernel"}
     users = {n for n in os.listdir(CSRC) if n.endswith((".cu", ".cuh")) and "team_rank()" in source(n)}
-    assert users >= {"constrain.cu", "row_team.cuh"}
+    assert users == {"constrain.cu", "distill.cu", "row_team.cuh"}
