@@ -6,10 +6,12 @@
 // and the listed ids are few.  So the sum leaves the listed ids out (no difference of nearly equal sums where the student is sure of the
 // list), the list's own terms and everything per row are taken in FP64 by few threads, and the gradient pass multiplies by one number.
 //
-// One team of up to eight CTAs per row, each with a slice of at most 64 KB that stays in shared memory: the row is read once, by
-// asynchronous copies into which each thread's own vectors come back to it (no barrier between copy and use), while the list is
-// gathered and reduced.  A running maximum and sum per thread, one exchange of (maximum, sum) between the CTAs, then the gradient from
-// shared memory.  Three CTAs share an SM, so that one reads while another writes.
+// A team of up to eight CTAs takes a row, each a slice of it that stays in shared memory, so that the row is read once, and goes on to
+// the next row of its own.  In a CTA, the compute warps run over the slice: a running maximum and sum per thread, one exchange of
+// (maximum, sum) between all warps of the team, then the gradient from shared memory.  A thread's vectors are its own from the
+// asynchronous copy on (no barrier between copy and use), and where it has written a vector's gradient it starts the copy of the
+// next row's.  Two more warps are a row ahead: one gathers and reduces the next row's list, the other sets the bits of the ids
+// that count into the sum and, a row behind, takes the loss in FP64.  Three CTAs share an SM, each at another point of its row.
 #include "packed_fma.cuh"
 #include "row_types.cuh"
 #include "row_team.cuh"
@@ -17,15 +19,16 @@
 #include "launch.h"
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 
 namespace ds41 {
 namespace {
 
 enum DistillMode { kDistillLoss, kDistillGrad, kDistillBoth };
-constexpr int kDisBytes = 65536;              // of a CTA's slice
-constexpr int kDisIds = kDisBytes / 2;
+constexpr int kDisSteps = 17;                 // vectors of a thread, the last one where a slice does not begin on a vector
+constexpr int kDisGroup = 4;                  // of them, those that are waited for together
 constexpr int kDisTop = DS41_B200_DISTILL_MAX_TOP;
-constexpr int kDisGroups = 8;                 // copies of a thread that are waited for one by one
+constexpr int kDisOwn = kDisTop / 32;         // entries of a lane
 constexpr double kDisMost = 1.01;             // what a list's probabilities may add up to: 1, and the rounding of stored values
 
 struct DistillParams {
@@ -38,7 +41,19 @@ __device__ __forceinline__ void copy16_async(const void *to, const void *from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kLeft> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+__device__ __forceinline__ void copies_wait(int left) {   // (a constant where it is called)
+  switch (left) {
+    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+    case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+    default: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+  }
+}
+template <int kBarrier, int kCount> __device__ __forceinline__ void barrier_of() {
+  __syncwarp();
+  asm volatile("bar.sync %0, %1;" ::"n"(kBarrier), "n"(kCount) : "memory");
+}
 
 __device__ __forceinline__ float exp2_approx(float x) {   // 2 ulp; 0 for -inf and below 2^-126
   float y;
@@ -46,365 +61,492 @@ __device__ __forceinline__ float exp2_approx(float x) {   // 2 ulp; 0 for -inf a
   return y;
 }
 
-// What the list amounts to, the same in every CTA of the team.
-struct ListSums {
-  double named, kept, entropy, share;         // sums of w over all entries in the vocabulary and over those that count, of
-};                                            // w (ln w - (z - zmax) / T), of exp((z - zmax) / T); one entry per id
-
-template <int kThreads>
+// What is known of a row besides its ids outside the list, the same in every CTA of the team.
+struct DistillRow {
+  float scale;
+  int reject;                                 // of the list
+  float4 stats;                               // of the forward pass, in the gradient's
+  float zmax, share;                          // largest logit of the entries that count; sum of exp((z - zmax) / T), an entry per id
+  double kept, entropy, rest;                 // with w the unnormalised weights: sum of w, of w (ln w - (z - zmax) / T); 1 - the list's sum
+  double inverse, inverse_rest;               // 1 / (sum of w), 1 / (that + rest)
+};
+template <int kCompute>
 struct DistillSmem {
-  uint32_t bits[kDisIds / 32 + 2];            // by place: allowed and not listed
-  int4 ids[kDisTop / 4];
-  double weights[kDisTop];
-  ListSums list[kThreads / 32];
-  float2 list_max[kThreads / 32];             // (largest value, largest logit) of the entries that count
-  float2 warp_sum[kThreads / 32];             // (maximum, sum) of the ids outside the list
-  float2 slot;                                // this CTA's, read by the others
-  double list_scale, log_sum;                 // of the row: what follows from all of it
-  double total, largest;
-  float coef, rest_max;
-  int reject;
+  DistillRow rows[4];                         // by the number of the row's turn: the last one, this one, the next two
+  float2 sums[2][kCompute / 32];              // every warp's (maximum, sum), read by the whole team
+  float2 result[2];                           // (maximum, sum) of the row's ids outside the list
 };
 
-template <class T, int kMode, int kThreads>
-__global__ void __launch_bounds__(kThreads, 1536 / kThreads) distill_kernel(DistillParams p) {
+// A row's slice as this CTA sees it.  Place 0 is where the vector of its first id begins.
+template <class T>
+struct DistillSlice {
+  const T *x;
+  int lead, vecs;
+  __device__ __forceinline__ DistillSlice(const DistillParams &p, int row, int begin, int len) {
+    x = static_cast<const T *>(p.a.logits) + size_t(row) * size_t(p.a.logits_stride) + begin;
+    lead = int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % RowType<T>::kVec);
+    vecs = (lead + len + RowType<T>::kVec - 1) / RowType<T>::kVec;
+  }
+};
+
+template <class T, int kMode, int kCompute>
+__global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distill_kernel(DistillParams p) {
   using R = RowType<T>;
-  constexpr int kVec = R::kVec, kWarps = kThreads / 32, kOwn = kDisTop / kThreads > 0 ? kDisTop / kThreads : 1;
+  constexpr int kVec = R::kVec, kWarps = kCompute / 32;
   constexpr unsigned kAll = (1u << kVec) - 1u;
-  extern __shared__ uint4 stage[];            // the slice, by vectors of the row: place 0 is where its first id's vector begins
-  __shared__ DistillSmem<kThreads> s;
+  extern __shared__ uint4 stage[];            // the slice, by vectors; behind it two rows' bits, weights, logits and ids of the list
+  __shared__ DistillSmem<kCompute> s;
+  const ds41_b200_distill_args &a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = int(blockIdx.x) / p.team, rank = int(team_rank());
-  const int begin = min(p.a.vocab, rank * p.slice), len = min(p.a.vocab - begin, p.slice);
+  const int rank = int(team_rank()), teams = int(gridDim.x) / p.team, own_team = int(blockIdx.x) / p.team;
+  const int begin = min(a.vocab, rank * p.slice), len = min(a.vocab - begin, p.slice);
+  const int top_room = (a.top + 3) & ~3, bits_room = p.slice / 32 + 2;
+  uint4 *const behind = stage + p.slice * int(sizeof(T)) / 16 + 1;
+  double *const weights = reinterpret_cast<double *>(behind);
+  int *const ids = reinterpret_cast<int *>(weights + 2 * top_room);
+  float *const zs = reinterpret_cast<float *>(ids + 2 * top_room);
+  uint32_t *const bits = reinterpret_cast<uint32_t *>(zs + 2 * top_room);   // by place: allowed and not listed
+  const double t = a.temperature;
   cudaGridDependencySynchronize();
   cudaTriggerProgrammaticLaunchCompletion();
 
-  const ds41_b200_distill_args &a = p.a;
-  const T *whole = static_cast<const T *>(a.logits) + size_t(row) * size_t(a.logits_stride), *x = whole + begin;
-  T *grad = kMode == kDistillLoss ? nullptr : static_cast<T *>(a.grad) + size_t(row) * size_t(a.grad_stride) + begin;
-  const uint32_t *mask = a.mask ? a.mask + size_t(row) * size_t(a.mask_stride) : nullptr;
-  const int lead = int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % kVec);
-  const int vecs = (lead + len + kVec - 1) / kVec;
-  const bool by_vectors = kMode != kDistillLoss && int((reinterpret_cast<uintptr_t>(grad) / sizeof(T)) % kVec) == lead;
-  auto partial = [&](int v) { return v * kVec < lead || (v + 1) * kVec > lead + len; };
-  // the gradient of vector v; ids outside the slice are not this CTA's
-  auto put = [&](int v, const uint4 &q) {
-    if (by_vectors && !partial(v)) {
-      reinterpret_cast<uint4 *>(grad - lead)[v] = q;
+  auto row_scale = [&](int row) { return kMode != kDistillLoss && a.row_scale && row < a.rows ? load_input(a.row_scale + row) : 1.f; };
+  auto skipped = [&](const DistillRow &r) { return kMode != kDistillLoss && r.scale == 0.f; };
+  auto partial = [&](const DistillSlice<T> &c, int v) { return v * kVec < c.lead || (v + 1) * kVec > c.lead + len; };
+  auto start_copy = [&](const DistillSlice<T> &c, int v) {   // a vector that is not whole comes by its ids
+    if (v >= c.vecs) return;
+    if (!partial(c, v)) {
+      copy16_async(&stage[v], reinterpret_cast<const uint4 *>(c.x - c.lead) + v);
     } else {
-      const T *each = reinterpret_cast<const T *>(&q);
-#pragma unroll
+      T *each = reinterpret_cast<T *>(&stage[v]);
       for (int k = 0; k < kVec; ++k) {
-        const int i = v * kVec + k - lead;
-        if (i >= 0 && i < len) grad[i] = each[k];
+        const int i = v * kVec + k - c.lead;
+        if (i >= 0 && i < len) each[k] = c.x[i];
       }
     }
   };
-  float scale = 1.f;
-  if (kMode != kDistillLoss && a.row_scale) {
-    scale = load_input(a.row_scale + row);
-    if (scale == 0.f) {                       // padding: the same in every CTA of the team
-      for (int v = tid; v < vecs; v += kThreads) put(v, make_uint4(0u, 0u, 0u, 0u));
-      if (kMode == kDistillBoth && rank == 0 && tid == 0) {
-        a.loss[row] = 0.f;
-        a.status[row] = 0;
-        if (a.stats) reinterpret_cast<float4 *>(a.stats)[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+
+  // ---- the list of the row of turn `turn`, by one warp
+  auto take_list = [&](int row, int turn) {
+    DistillRow &r = s.rows[turn & 3];
+    double *const w_list = weights + (turn & 1) * top_room;
+    int *const id_list = ids + (turn & 1) * top_room;
+    float *const z_list = zs + (turn & 1) * top_room;
+    const T *whole = static_cast<const T *>(a.logits) + size_t(row) * size_t(a.logits_stride);
+    const uint32_t *mask = a.mask ? a.mask + size_t(row) * size_t(a.mask_stride) : nullptr;
+    const int own = (a.top + 31) / 32;
+    unsigned named = 0u, counts = 0u;         // a bit per entry of the lane
+    bool bad = false;
+    float most = -FLT_MAX, zmax = -FLT_MAX;
+    for (int k = 0; k < own; ++k) {
+      const int e = lane + 32 * k;
+      int id = -1;
+      double value = 0.0;
+      float z = 0.f;
+      if (e < a.top) {
+        id = load_input(a.teacher_ids + size_t(row) * size_t(a.ids_stride) + e);
+        const size_t at = size_t(row) * size_t(a.values_stride) + e;
+        value = a.teacher_dtype == DS41_B200_F64 ? load_input(static_cast<const double *>(a.teacher_values) + at)
+                                                 : double(load_input(static_cast<const float *>(a.teacher_values) + at));
       }
+      if (id >= 0 && id < a.vocab) {
+        named |= 1u << k;
+        bad |= !(value < INFINITY);
+        if (!mask || ((load_input(mask + (id >> 5)) >> (id & 31)) & 1u)) {
+          z = R::load(whole[id]);
+          bad |= !(z < INFINITY);
+          if (!(z == -INFINITY)) { counts |= 1u << k; most = fmaxf(most, float(value)); zmax = fmaxf(zmax, z); }
+        }
+      }
+      if (e < top_room) { id_list[e] = (counts >> k) & 1u ? id : -2 - e; w_list[e] = value; z_list[e] = z; }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      zmax = fmaxf(zmax, __shfl_xor_sync(0xffffffffu, zmax, o));
+    }
+    __syncwarp();
+    unsigned first = counts;                  // entries with no other of the same id in front of them
+    for (int k = 0; k < own; ++k) {
+      if (!((counts >> k) & 1u)) continue;
+      const int e = lane + 32 * k, id = id_list[e];
+      for (int j = 0; 4 * j < e; ++j) {
+        const int4 q = reinterpret_cast<const int4 *>(id_list)[j];
+        const int before = e - 4 * j;
+        if (q.x == id || (before > 1 && q.y == id) || (before > 2 && q.z == id) || (before > 3 && q.w == id)) { first &= ~(1u << k); break; }
+      }
+    }
+    const bool again = __any_sync(0xffffffffu, first != counts);
+    double list = 0.0, kept = 0.0, entropy = 0.0;
+    float share = 0.f;
+    for (int k = 0; k < own; ++k) {
+      const int e = lane + 32 * k;
+      if (!((named >> k) & 1u)) continue;
+      const double log_w = a.tail ? w_list[e] : (w_list[e] - double(most)) / t, w = exp(log_w);
+      list += w;
+      const bool is = (counts >> k) & 1u;
+      w_list[e] = is ? w : 0.0;
+      if (!is) continue;
+      kept += w;
+      if (!again) {
+        const double gap = (double(z_list[e]) - double(zmax)) / t;
+        if (w > 0.0) entropy += w * (log_w - gap);
+        share += exp2_approx((z_list[e] - zmax) * p.log2e_t);
+      }
+    }
+    if (again) {                              // an id's first entry takes the weights of the later ones
+      __syncwarp();
+      double merged[kDisOwn];
+      for (int k = 0; k < own; ++k) {
+        const int e = lane + 32 * k;
+        merged[k] = e < a.top ? w_list[e] : 0.0;
+        if (!((first >> k) & 1u)) continue;
+        for (int j = e + 1; j < a.top; ++j)
+          if (id_list[j] == id_list[e]) merged[k] += w_list[j];
+        const double gap = (double(z_list[e]) - double(zmax)) / t;
+        if (merged[k] > 0.0) entropy += merged[k] * (log(merged[k]) - gap);
+        share += exp2_approx((z_list[e] - zmax) * p.log2e_t);
+      }
+      __syncwarp();
+      for (int k = 0; k < own; ++k) {
+        const int e = lane + 32 * k;
+        if (e >= a.top) continue;
+        w_list[e] = merged[k];
+        if (((counts & ~first) >> k) & 1u) id_list[e] = -2 - e;
+      }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      list += __shfl_xor_sync(0xffffffffu, list, o);
+      kept += __shfl_xor_sync(0xffffffffu, kept, o);
+      entropy += __shfl_xor_sync(0xffffffffu, entropy, o);
+      share += __shfl_xor_sync(0xffffffffu, share, o);
+    }
+    bad = __any_sync(0xffffffffu, bad);
+    if (lane == 0) {
+      r.reject = bad ? DS41_B200_ROW_NONFINITE : a.tail && list > kDisMost ? DS41_B200_ROW_NOT_NORMALIZED : !(kept > 0.0) ? DS41_B200_ROW_EMPTY : 0;
+      r.zmax = zmax; r.share = share; r.kept = kept; r.entropy = entropy;
+      r.rest = a.tail ? fmax(0.0, 1.0 - list) : 0.0;
+      r.inverse = 1.0 / kept; r.inverse_rest = 1.0 / (kept + r.rest);
+      if (kMode == kDistillGrad) r.stats = reinterpret_cast<const float4 *>(a.stats)[row];
+    }
+    barrier_of<2, 64>();                      // (the bits are set)
+    const DistillSlice<T> c(p, row, begin, len);
+    uint32_t *const out = bits + (turn & 1) * bits_room;
+    for (int k = 0; k < own; ++k) {
+      const int e = lane + 32 * k;
+      const unsigned local = e < a.top ? unsigned(id_list[e]) - unsigned(begin) : ~0u;
+      if (local < unsigned(len)) {
+        const unsigned place = local + unsigned(c.lead);
+        atomicAnd(&out[place >> 5], ~(1u << (place & 31u)));
+      }
+    }
+  };
+  // ---- by the other: the bits of its allowed ids
+  auto take_bits = [&](int row, int turn) {
+    const DistillSlice<T> c(p, row, begin, len);
+    uint32_t *const out = bits + (turn & 1) * bits_room;
+    const uint32_t *mask = a.mask ? a.mask + size_t(row) * size_t(a.mask_stride) : nullptr;
+    const int first = begin / 32, words = (a.vocab + 31) / 32;
+    auto word = [&](int at) { return at >= 0 && at < words ? load_input(mask + at) : 0u; };
+#pragma unroll 8
+    for (int w = lane; w <= (c.lead + len) / 32; w += 32) {
+      uint32_t in = ~0u;
+      if (mask) {
+        in = word(first + w);
+        if (c.lead) in = in << c.lead | word(first + w - 1) >> (32 - c.lead);
+      }
+      const int low = c.lead - 32 * w, high = c.lead + len - 32 * w;  // of the slice's places
+      if (low > 0) in &= low < 32 ? ~0u << low : 0u;
+      if (high < 32) in &= high > 0 ? (1u << high) - 1u : 0u;
+      out[w] = in;
+    }
+    barrier_of<2, 64>();
+  };
+  // ---- loss, stats and status of a row that is done
+  auto finish = [&](int row, int turn) {
+    const DistillRow &r = s.rows[turn & 3];
+    if (skipped(r)) {
+      a.loss[row] = 0.f; a.status[row] = 0;
+      if (a.stats) reinterpret_cast<float4 *>(a.stats)[row] = make_float4(0.f, 0.f, 0.f, 0.f);
       return;
     }
-  }
-
-  // ---- the slice on its way; a vector that is not whole comes by its ids
-#pragma unroll
-  for (int g = 0; g < kDisGroups; ++g) {
-    for (int v = tid + g * kThreads; v < vecs; v += g < kDisGroups - 1 ? vecs : kThreads) {
-      if (partial(v)) {
-        T *each = reinterpret_cast<T *>(&stage[v]);
-        for (int k = 0; k < kVec; ++k) {
-          const int i = v * kVec + k - lead;
-          if (i >= 0 && i < len) each[k] = x[i];
-        }
-      } else {
-        copy16_async(&stage[v], reinterpret_cast<const uint4 *>(x - lead) + v);
-      }
+    const float rest_max = s.result[turn & 1].x, rest_sum = s.result[turn & 1].y, nan = __int_as_float(0x7fffffff);
+    const int reject = r.reject ? r.reject : rest_sum < INFINITY ? 0 : DS41_B200_ROW_NONFINITE;
+    float loss = reject == DS41_B200_ROW_EMPTY ? 0.f : nan;
+    float4 stats = make_float4(nan, nan, nan, nan);
+    if (!reject) {
+      const bool any = rest_sum != 0.f;
+      const double zmax = r.zmax, largest = any ? fmax(double(rest_max), zmax) : zmax;
+      const double log_rest = log(double(rest_sum));
+      const double log_sum = log((any ? double(rest_sum) * exp((double(rest_max) - largest) / t) : 0.0) + double(r.share) * exp((zmax - largest) / t));
+      const double inverse = any ? r.inverse_rest : r.inverse, kept = r.kept * inverse, tail = any ? r.rest * inverse : 0.0;
+      double sum = r.entropy * inverse + kept * (log(inverse) + log_sum - (zmax - largest) / t);
+      if (tail > 0.0) sum += tail * (log(tail) - ((double(rest_max) - largest) / t + log_rest - log_sum));
+      loss = float(t * t * sum);
+      stats = make_float4(float(largest), float(log_sum), any ? rest_max : -INFINITY, any ? float(log_rest) : -INFINITY);
     }
-    copies_commit();
-  }
-
-  // ---- the list: what counts of it, and where it lies
-  for (int w = tid; w <= (lead + len) / 32; w += kThreads) {
-    uint32_t in = ~0u;
-    if (mask) {
-      const int first = begin / 32, words = (a.vocab + 31) / 32;
-      auto word = [&](int at) { return at >= 0 && at < words ? load_input(mask + at) : 0u; };
-      in = lead ? word(first + w) << lead | word(first + w - 1) >> (32 - lead) : word(first + w);
-    }
-    const int low = lead - 32 * w, high = lead + len - 32 * w;        // of the slice's places
-    if (low > 0) in &= low < 32 ? ~0u << low : 0u;
-    if (high < 32) in &= high > 0 ? (1u << high) - 1u : 0u;
-    s.bits[w] = in;
-  }
-  int id[kOwn];
-  float z[kOwn];
-  double value[kOwn], weight[kOwn];
-  bool counts[kOwn], named[kOwn], bad = false;
-  float most = -FLT_MAX, zmax = -FLT_MAX;
-#pragma unroll
-  for (int k = 0; k < kOwn; ++k) {
-    const int e = tid + k * kThreads;
-    id[k] = -1; z[k] = 0.f; value[k] = 0.0; weight[k] = 0.0;
-    if (e < a.top) {
-      id[k] = load_input(a.teacher_ids + size_t(row) * size_t(a.ids_stride) + e);
-      const size_t at = size_t(row) * size_t(a.values_stride) + e;
-      value[k] = a.teacher_dtype == DS41_B200_F64 ? load_input(static_cast<const double *>(a.teacher_values) + at)
-                                                  : double(load_input(static_cast<const float *>(a.teacher_values) + at));
-    }
-    named[k] = id[k] >= 0 && id[k] < a.vocab;
-    counts[k] = named[k] && (!mask || ((load_input(mask + (id[k] >> 5)) >> (id[k] & 31)) & 1u));
-    if (counts[k]) z[k] = R::load(whole[id[k]]);
-    counts[k] = counts[k] && !(z[k] == -INFINITY);
-    bad |= named[k] && !(value[k] < INFINITY);
-    bad |= counts[k] && !(z[k] < INFINITY);
-    if (counts[k]) { most = fmaxf(most, float(value[k])); zmax = fmaxf(zmax, z[k]); }
-    if (e < kDisTop) reinterpret_cast<int *>(s.ids)[e] = counts[k] ? id[k] : -2 - e;
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    zmax = fmaxf(zmax, __shfl_xor_sync(0xffffffffu, zmax, o));
-  }
-  if (lane == 0) s.list_max[warp] = make_float2(most, zmax);
-  bad = __syncthreads_or(int(bad));
-  for (int w = 0; w < kWarps; ++w) { most = fmaxf(most, s.list_max[w].x); zmax = fmaxf(zmax, s.list_max[w].y); }
-  const double t = a.temperature;
-  bool first[kOwn], again = false;
-#pragma unroll
-  for (int k = 0; k < kOwn; ++k) {
-    const int e = tid + k * kThreads;
-    first[k] = counts[k];
-    if (named[k]) weight[k] = a.tail ? exp(value[k]) : exp((value[k] - double(most)) / t);
-    if (counts[k]) {
-      for (int j = 0; 4 * j < e; ++j) {       // an entry of the same id in front of it?
-        const int4 q = s.ids[j];
-        const int before = e - 4 * j;
-        if (q.x == id[k] || (before > 1 && q.y == id[k]) || (before > 2 && q.z == id[k]) || (before > 3 && q.w == id[k])) first[k] = false;
-      }
-      again |= !first[k];
-      const unsigned local = unsigned(id[k]) - unsigned(begin);
-      if (local < unsigned(len)) {
-        const unsigned place = local + unsigned(lead);
-        atomicAnd(&s.bits[place >> 5], ~(1u << (place & 31u)));
-      }
-    }
-    if (e < kDisTop) s.weights[e] = counts[k] ? weight[k] : 0.0;
-  }
-  again = __syncthreads_or(int(again));
-  ListSums sums{0.0, 0.0, 0.0, 0.0};
-#pragma unroll
-  for (int k = 0; k < kOwn; ++k) {
-    sums.named += weight[k];
-    if (!first[k]) continue;
-    if (again) {
-      const int *ids = reinterpret_cast<const int *>(s.ids);
-      for (int j = tid + k * kThreads + 1; j < a.top; ++j)
-        if (ids[j] == id[k]) weight[k] += s.weights[j];
-    }
-    const double gap = (double(z[k]) - double(zmax)) / t;
-    sums.kept += weight[k];
-    if (weight[k] > 0.0) sums.entropy += weight[k] * (log(weight[k]) - gap);
-    sums.share += exp(gap);
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    sums.named += __shfl_xor_sync(0xffffffffu, sums.named, o);
-    sums.kept += __shfl_xor_sync(0xffffffffu, sums.kept, o);
-    sums.entropy += __shfl_xor_sync(0xffffffffu, sums.entropy, o);
-    sums.share += __shfl_xor_sync(0xffffffffu, sums.share, o);
-  }
-  if (lane == 0) s.list[warp] = sums;
-
-  // ---- maximum and sum of the ids outside the list; what is left out becomes -inf in shared memory
-  const float2x c2 = pack_f32x2(p.log2e_t, p.log2e_t);
-  float high = -FLT_MAX;
-  float2x sum2 = pack_f32x2(0.f, 0.f);
-  auto take = [&](int v) {
-    float y[kVec];
-    R::unpack(stage[v], y);
-    const unsigned in = (s.bits[v * kVec >> 5] >> (v * kVec & 31)) & kAll;
-    if (in != kAll) {
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) y[k] = (in >> k) & 1u ? y[k] : -INFINITY;
-      stage[v] = R::pack(y);
-    }
-    if (kMode == kDistillGrad) return;
-    float top = y[0];
-#pragma unroll
-    for (int k = 1; k < kVec; ++k) top = fmaxf(top, y[k]);
-    if (top > high) {
-      const float down = exp2_approx((high - top) * p.log2e_t);
-      sum2 = mul_f32x2(sum2, pack_f32x2(down, down));
-      high = top;
-    }
-    const float2x minus = pack_f32x2(-high, -high);
-#pragma unroll
-    for (int k = 0; k < kVec; k += 2) {
-      float e0, e1;
-      unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(y[k], y[k + 1]), minus), c2), e0, e1);
-      sum2 = add_f32x2(sum2, pack_f32x2(exp2_approx(e0), exp2_approx(e1)));
-    }
+    a.loss[row] = loss;
+    a.status[row] = reject;
+    if (a.stats) reinterpret_cast<float4 *>(a.stats)[row] = stats;
   };
+
+  // ---- the first row on its way
+  if (warp < kWarps) {
+    if (row_scale(own_team) != 0.f) {
+      const DistillSlice<T> c(p, own_team, begin, len);
 #pragma unroll
-  for (int g = 0; g < kDisGroups; ++g) {
-    if (g == 0) copies_wait<7>();
-    if (g == 1) copies_wait<6>();
-    if (g == 2) copies_wait<5>();
-    if (g == 3) copies_wait<4>();
-    if (g == 4) copies_wait<3>();
-    if (g == 5) copies_wait<2>();
-    if (g == 6) copies_wait<1>();
-    if (g == 7) copies_wait<0>();
-    for (int v = tid + g * kThreads; v < vecs; v += g < kDisGroups - 1 ? vecs : kThreads) take(v);
-  }
-  if (kMode != kDistillGrad) {
-    float s0, s1, all = high;
-    unpack_f32x2(sum2, s0, s1);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
-    float sum = (s0 + s1) * exp2_approx((high - all) * p.log2e_t);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) s.warp_sum[warp] = make_float2(all, sum);
-    __syncthreads();
-    if (warp == 0) {
-      const float2 own = lane < kWarps ? s.warp_sum[lane] : make_float2(-FLT_MAX, 0.f);
-      all = own.x;
-#pragma unroll
-      for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
-      sum = own.y * exp2_approx((own.x - all) * p.log2e_t);
-#pragma unroll
-      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0) s.slot = make_float2(all, sum);
-    }
-  }
-  team_barrier();                             // every CTA has its slot, and has read of the row what it needs of other slices
-  // ---- what follows for the row, by one warp of each CTA
-  if (warp == 0) {
-    ListSums list{0.0, 0.0, 0.0, 0.0};
-    for (int w = 0; w < kWarps; ++w) {
-      list.named += s.list[w].named; list.kept += s.list[w].kept;
-      list.entropy += s.list[w].entropy; list.share += s.list[w].share;
-    }
-    float rest_max = -FLT_MAX, rest_sum = 0.f;
-    double largest, log_sum, log_rest;        // (log_rest: of the sum outside the list, relative to rest_max)
-    bool any;
-    if (kMode == kDistillGrad) {
-      const float4 kept = reinterpret_cast<const float4 *>(a.stats)[row];
-      rest_sum = kept.x == kept.x ? 0.f : kept.x;   // (NaN: the forward pass has rejected the row)
-      any = kept.w > -INFINITY;
-      largest = kept.x; log_sum = kept.y; rest_max = any ? kept.z : 0.f; log_rest = kept.w;
-    } else {
-      const float2 its = lane < p.team ? team_read(&s.slot, lane) : make_float2(-FLT_MAX, 0.f);
-      rest_max = its.x;
-#pragma unroll
-      for (int o = 4; o; o >>= 1) rest_max = fmaxf(rest_max, __shfl_xor_sync(0xffffffffu, rest_max, o));
-      rest_sum = its.y * exp2_approx((its.x - rest_max) * p.log2e_t);
-#pragma unroll
-      for (int o = 4; o; o >>= 1) rest_sum += __shfl_xor_sync(0xffffffffu, rest_sum, o);
-      any = !(rest_sum == 0.f);
-      if (!any) rest_max = -FLT_MAX;
-    }
-    if (lane == 0) {
-      if (kMode != kDistillGrad) {
-        largest = any ? double(fmaxf(rest_max, zmax)) : double(zmax);
-        log_rest = log(double(rest_sum));
-        log_sum = log((any ? double(rest_sum) * exp((double(rest_max) - largest) / t) : 0.0) + list.share * exp((double(zmax) - largest) / t));
-      }
-      int reject = 0;
-      if (bad) reject = DS41_B200_ROW_NONFINITE;
-      else if (a.tail && list.named > kDisMost) reject = DS41_B200_ROW_NOT_NORMALIZED;
-      else if (!(list.kept > 0.0)) reject = DS41_B200_ROW_EMPTY;
-      else if (!(rest_sum < INFINITY)) reject = DS41_B200_ROW_NONFINITE;
-      const double rest = a.tail && any ? fmax(0.0, 1.0 - list.named) : 0.0, total = list.kept + rest, tail = rest / total;
-      const double log_q = any ? (double(rest_max) - largest) / t + log_rest - log_sum : 0.0;
-      const double q_rest = any ? exp(log_q) : 0.0;
-      s.coef = any ? float(double(scale) * t * (q_rest - tail) * exp(-log_rest)) : 0.f;
-      s.rest_max = rest_max;
-      s.list_scale = double(scale) * t;
-      s.total = total; s.largest = largest; s.log_sum = log_sum;
-      s.reject = reject;
-      if (kMode != kDistillGrad && rank == 0) {
-        const double kept = list.kept / total;
-        double loss = list.entropy / total - kept * log(total) - kept * ((double(zmax) - largest) / t - log_sum);
-        if (tail > 0.0) loss += tail * (log(tail) - log_q);
-        const float nan = __int_as_float(0x7fffffff);
-        a.loss[row] = reject == 0 ? float(t * t * loss) : reject == DS41_B200_ROW_EMPTY ? 0.f : nan;
-        a.status[row] = reject;
-        if (a.stats)
-          reinterpret_cast<float4 *>(a.stats)[row] = reject ? make_float4(nan, nan, nan, nan)
-            : make_float4(float(largest), float(log_sum), any ? rest_max : -INFINITY, any ? float(log_rest) : -INFINITY);
+      for (int g = 0; g < kDisSteps; ++g) {
+        start_copy(c, tid + g * kCompute);
+        if (g % kDisGroup == kDisGroup - 1 || g == kDisSteps - 1) copies_commit();
       }
     }
+  } else if (warp == kWarps) {
+    take_list(own_team, 0);
+  } else {
+    if (lane < 2) s.rows[lane].scale = row_scale(own_team + lane * teams);
+    take_bits(own_team, 0);
   }
-  team_arrive();                              // (the slots have been read)
-  if (kMode != kDistillLoss) {
-    __syncthreads();
-    const int reject = s.reject;
-    if (reject) {
-      const T nan = R::store(__int_as_float(0x7fffffff));
-      T each[kVec];
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) each[k] = nan;
-      const uint4 q = reject == DS41_B200_ROW_EMPTY ? make_uint4(0u, 0u, 0u, 0u) : *reinterpret_cast<const uint4 *>(each);
-      for (int v = tid; v < vecs; v += kThreads) put(v, q);
+  __syncthreads();
+
+  int turn = 0;
+  for (int row = own_team; row < a.rows; row += teams, ++turn) {
+    const int next = row + teams;
+    if (warp >= kWarps) {                     // a row ahead
+      if (p.team > 1) team_arrive();
+      if (warp == kWarps) {
+        if (next < a.rows) take_list(next, turn + 1);
+      } else {
+        if (lane == 0) s.rows[(turn + 2) & 3].scale = row_scale(next + teams);
+        if (next < a.rows) take_bits(next, turn + 1);
+        if (kMode != kDistillGrad && rank == 0 && lane == 0 && turn > 0) finish(row - teams, turn - 1);
+      }
+      if (p.team > 1) team_wait();
     } else {
-      const float2x minus = pack_f32x2(-s.rest_max, -s.rest_max), coef2 = pack_f32x2(s.coef, s.coef);
-      for (int v = tid; v < vecs; v += kThreads) {
-        float y[kVec];
+      const DistillRow &r = s.rows[turn & 3];
+      const DistillSlice<T> c(p, row, begin, len), c_next(p, next < a.rows ? next : row, begin, len);
+      const bool skip = skipped(r), ahead = next < a.rows && !skipped(s.rows[(turn + 1) & 3]);
+      const uint32_t *const in_sum = bits + (turn & 1) * bits_room;
+      const float2x c2 = pack_f32x2(p.log2e_t, p.log2e_t);
+      T *const grad = kMode == kDistillLoss ? nullptr : static_cast<T *>(a.grad) + size_t(row) * size_t(a.grad_stride) + begin;
+      const bool by_vectors = kMode != kDistillLoss && int((reinterpret_cast<uintptr_t>(grad) / sizeof(T)) % kVec) == c.lead;
+      // the vector's ids that are in the sum; the others are -inf
+      auto values = [&](int v, float (&y)[kVec]) {
         R::unpack(stage[v], y);
+        const unsigned in = (in_sum[v * kVec >> 5] >> (v * kVec & 31)) & kAll;
+        if (in == kAll) return false;
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) y[k] = (in >> k) & 1u ? y[k] : -INFINITY;
+        return true;
+      };
+      auto put = [&](int v, const uint4 &q) {
+        if (by_vectors && !partial(c, v)) {
+          reinterpret_cast<uint4 *>(grad - c.lead)[v] = q;
+        } else {
+          const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int k = 0; k < kVec; ++k) {
+            const int i = v * kVec + k - c.lead;
+            T each;
+            if constexpr (sizeof(T) == 4) each = __uint_as_float(w[k]);
+            else *reinterpret_cast<uint16_t *>(&each) = uint16_t(w[k / 2] >> (k % 2 * 16));
+            if (i >= 0 && i < len) grad[i] = each;
+          }
+        }
+      };
+      // f(v) over the thread's vectors; kArrive: as their copies arrive; kNext: behind each the copy of the next row's
+      auto run = [&](auto arrive, auto start_next, auto f) {
+#pragma unroll
+        for (int g = 0; g < kDisSteps; ++g) {
+          // (with a group of the next row's behind each of this one's, the newest four may always be on their way)
+          if (arrive.value && g % kDisGroup == 0) copies_wait((kDisSteps - 1) / kDisGroup - (start_next.value && ahead ? 0 : g / kDisGroup));
+          const int v = tid + g * kCompute;
+          if (v < c.vecs) f(v);
+          if (start_next.value && ahead) {
+            start_copy(c_next, v);
+            if (g % kDisGroup == kDisGroup - 1 || g == kDisSteps - 1) copies_commit();
+          }
+        }
+      };
+      using Yes = std::true_type;
+      using No = std::false_type;
+
+      // ---- maximum and sum of the ids outside the list
+      float high = -FLT_MAX;
+      float2x sum2 = pack_f32x2(0.f, 0.f);
+      auto add = [&](int v) {
+        float y[kVec];
+        const bool changed = values(v, y);
+        if (kMode == kDistillBoth && changed) stage[v] = R::pack(y);
+        float top = y[0];
+#pragma unroll
+        for (int k = 1; k < kVec; ++k) top = fmaxf(top, y[k]);
+        if (top > high) {
+          const float down = exp2_approx((high - top) * p.log2e_t);
+          sum2 = mul_f32x2(sum2, pack_f32x2(down, down));
+          high = top;
+        }
+        const float2x minus = pack_f32x2(-high, -high);
 #pragma unroll
         for (int k = 0; k < kVec; k += 2) {
           float e0, e1;
           unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(y[k], y[k + 1]), minus), c2), e0, e1);
-          unpack_f32x2(mul_f32x2(pack_f32x2(exp2_approx(e0), exp2_approx(e1)), coef2), y[k], y[k + 1]);
+          sum2 = add_f32x2(sum2, pack_f32x2(exp2_approx(e0), exp2_approx(e1)));
         }
-        put(v, R::pack(y));
-      }
-      __syncthreads();                        // (zeros stand where listed ids are)
+      };
+      if (kMode == kDistillLoss) run(Yes{}, Yes{}, add);
+      if (kMode == kDistillBoth && !skip) run(Yes{}, No{}, add);
+      if (kMode != kDistillGrad) {
+        float s0, s1, all = high;
+        unpack_f32x2(sum2, s0, s1);
 #pragma unroll
-      for (int k = 0; k < kOwn; ++k) {
-        const unsigned local = unsigned(id[k]) - unsigned(begin);
-        if (first[k] && local < unsigned(len)) {
-          const double q = exp((double(z[k]) - s.largest) / t - s.log_sum);
-          grad[local] = R::store(float(s.list_scale * (q - weight[k] / s.total)));
+        for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
+        float sum = (s0 + s1) * exp2_approx((high - all) * p.log2e_t);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) s.sums[turn & 1][warp] = make_float2(all, sum);
+      }
+      if (p.team > 1) team_barrier();         // every CTA has its sums, and has read of the row what it needs of other slices
+      else barrier_of<1, kCompute>();
+      float rest_max = -FLT_MAX, rest_sum = 0.f;
+      if (kMode != kDistillGrad) {
+        for (int w = lane; w < kWarps * p.team; w += 32) {            // (64 at most: two a lane, of the same order everywhere)
+          const float2 its = team_read(&s.sums[turn & 1][w % kWarps], w / kWarps);
+          const float most = fmaxf(rest_max, its.x);
+          rest_sum = rest_sum * exp2_approx((rest_max - most) * p.log2e_t) + its.y * exp2_approx((its.x - most) * p.log2e_t);
+          rest_max = most;
+        }
+        float all = rest_max;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
+        rest_sum *= exp2_approx((rest_max - all) * p.log2e_t);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) rest_sum += __shfl_xor_sync(0xffffffffu, rest_sum, o);
+        rest_max = all;
+        if (tid == 0) s.result[turn & 1] = make_float2(rest_max, rest_sum);
+      }
+
+      // ---- the gradient
+      if (kMode != kDistillLoss) {
+        float largest, inverse_sum, q_rest;   // of all ids: the maximum, 1 / the sum; share of the ids outside the list
+        bool any;
+        int reject = r.reject;
+        if (kMode == kDistillGrad) {
+          largest = r.stats.x; inverse_sum = exp2_approx(-r.stats.y * 1.44269504f);
+          any = r.stats.w > -INFINITY;
+          rest_max = any ? r.stats.z : 0.f;
+          rest_sum = any ? exp2_approx(r.stats.w * 1.44269504f) : 0.f;
+          q_rest = any ? rest_sum * exp2_approx((rest_max - largest) * p.log2e_t) * inverse_sum : 0.f;
+          if (!reject && !(r.stats.x == r.stats.x)) reject = DS41_B200_ROW_NONFINITE;
+        } else {
+          any = rest_sum != 0.f;
+          largest = any ? fmaxf(rest_max, r.zmax) : r.zmax;
+          const float part = any ? rest_sum * exp2_approx((rest_max - largest) * p.log2e_t) : 0.f;
+          inverse_sum = 1.f / (part + r.share * exp2_approx((r.zmax - largest) * p.log2e_t));
+          q_rest = part * inverse_sum;
+          if (!reject && !(rest_sum < INFINITY)) reject = DS41_B200_ROW_NONFINITE;
+        }
+        const double inverse = any ? r.inverse_rest : r.inverse;
+        const double factor = double(r.scale) * t;
+        const float tail = any ? float(r.rest * inverse) : 0.f, coef = any ? float(factor) * (q_rest - tail) / rest_sum : 0.f;
+        if (skip || reject) {
+          const T nan = R::store(__int_as_float(0x7fffffff));
+          uint32_t w = 0u;
+          if (!skip && reject != DS41_B200_ROW_EMPTY)
+            w = sizeof(T) == 4 ? *reinterpret_cast<const uint32_t *>(&nan) : *reinterpret_cast<const uint16_t *>(&nan) * 0x10001u;
+          const uint4 q = make_uint4(w, w, w, w);
+          if (!skip) copies_wait(0);
+          run(No{}, Yes{}, [&](int v) { put(v, q); });
+        } else {
+          const float2x minus = pack_f32x2(-rest_max, -rest_max), coef2 = pack_f32x2(coef, coef);
+          auto step = [&](int v) {
+            float y[kVec];
+            if (kMode == kDistillGrad) values(v, y);
+            else R::unpack(stage[v], y);
+#pragma unroll
+            for (int k = 0; k < kVec; k += 2) {
+              float e0, e1;
+              unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(y[k], y[k + 1]), minus), c2), e0, e1);
+              unpack_f32x2(mul_f32x2(pack_f32x2(exp2_approx(e0), exp2_approx(e1)), coef2), y[k], y[k + 1]);
+            }
+            put(v, R::pack(y));
+          };
+          if (kMode == kDistillGrad) run(Yes{}, Yes{}, step);
+          else run(No{}, Yes{}, step);
+          barrier_of<1, kCompute>();          // (zeros stand where listed ids are)
+          for (int e = tid; e < a.top; e += kCompute) {
+            const unsigned local = unsigned(ids[(turn & 1) * top_room + e]) - unsigned(begin);
+            if (local >= unsigned(len)) continue;
+            const float q = exp2_approx((zs[(turn & 1) * top_room + e] - largest) * p.log2e_t) * inverse_sum;
+            grad[local] = R::store(float(factor * (double(q) - weights[(turn & 1) * top_room + e] * inverse)));
+          }
         }
       }
     }
+    __syncthreads();
   }
-  team_wait();
+  if (kMode != kDistillGrad && rank == 0 && tid == kCompute + 32) finish(own_team + (turn - 1) * teams, turn - 1);
+  if (p.team > 1) team_barrier();
 }
 
-template <class T, int kMode, int kThreads>
+// Teams that the GPU holds at a time (asked of the runtime once per variant, device, team and shared memory of a thread's calls).
+template <class T, int kMode, int kCompute>
+cudaError_t resident_teams(const cudaLaunchConfig_t &cfg, int dev, int team, int *teams) {
+  static thread_local struct { int dev, team, teams; size_t smem; } known{-1, 0, 0, 0};
+  if (known.dev != dev) {
+    const cudaError_t e = cudaFuncSetAttribute(distill_kernel<T, kMode, kCompute>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+    if (e != cudaSuccess) return e;
+  }
+  if (known.dev != dev || known.team != team || known.smem != cfg.dynamicSmemBytes) {
+    int n = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, distill_kernel<T, kMode, kCompute>, &cfg);
+    if (e != cudaSuccess) return e;
+    known = {dev, team, n < 1 ? 1 : n, cfg.dynamicSmemBytes};
+  }
+  *teams = known.teams;
+  return cudaSuccess;
+}
+
+size_t distill_smem(int slice, int top, size_t bytes) {
+  return size_t(slice) * bytes + 16 + 2 * size_t((top + 3) & ~3) * 16 + 2 * (size_t(slice) / 32 + 2) * 4;
+}
+
+template <class T, int kMode, int kCompute>
 cudaError_t launch_distill(const DistillParams &p, cudaStream_t stream) {
-  static thread_local int configured_device = -1;
-  int dev = 0;
+  int dev = 0, teams = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (configured_device != dev) {
-    e = cudaFuncSetAttribute(distill_kernel<T, kMode, kThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize, kDisBytes + 16);
-    if (e != cudaSuccess) return e;
-    configured_device = dev;
-  }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(p.a.rows) * unsigned(p.team));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = size_t(p.slice) * sizeof(T) + 16;
+  cfg.gridDim = dim3(unsigned(p.team));
+  cfg.blockDim = dim3(kCompute + 64);
+  cfg.dynamicSmemBytes = distill_smem(p.slice, p.a.top, sizeof(T));
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = unsigned(p.team); attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   attr[1] = programmatic_launch();
-  cfg.attrs = attr; cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, distill_kernel<T, kMode, kThreads>, p);
+  cfg.attrs = attr; cfg.numAttrs = 1;
+  e = resident_teams<T, kMode, kCompute>(cfg, dev, p.team, &teams);
+  if (e != cudaSuccess) return e;
+  // as many rows for every team, if not one less
+  const int turns = (p.a.rows + teams - 1) / teams;
+  cfg.gridDim = dim3(unsigned((p.a.rows + turns - 1) / turns) * unsigned(p.team));
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, distill_kernel<T, kMode, kCompute>, p);
+}
+
+template <class T, int kMode>
+cudaError_t launch_distill(DistillParams &d, cudaStream_t stream) {
+  constexpr int kSmall = 64 * (kDisSteps - 1) * 16 / int(sizeof(T)), kLarge = 4 * kSmall;   // ids of a CTA
+  const int vocab = d.a.vocab, top = d.a.top;
+  // CTAs per row: as few as hold it, three CTAs to an SM where eight of them can, and for batches that leave SMs idle up to eight, of at least
+  // 4096 ids each
+  auto slice = [&](int team) { return ((vocab + team - 1) / team + 31) & ~31; };
+  d.team = 1;
+  while (d.team < 8 && (slice(d.team) > kLarge || distill_smem(slice(d.team), top, sizeof(T)) > 74 * 1024)) ++d.team;
+  while (d.team < 8 && 2LL * d.a.rows * d.team <= 148 && vocab > d.team * 4096) ++d.team;
+  d.slice = slice(d.team);
+  return d.slice <= kSmall ? launch_distill<T, kMode, 64>(d, stream) : launch_distill<T, kMode, 256>(d, stream);
 }
 
 template <int kMode>
@@ -436,15 +578,10 @@ int distill(const ds41_b200_distill_args *p, cudaStream_t stream) {
       return invalid("distill args: grad overlaps logits without being the same rows");
   }
   DistillParams d{*p, 0, 1, float(1.4426950408889634 / p->temperature)};
-  // CTAs per row: as few as hold it, and for batches that leave SMs idle up to eight, of at least 4096 ids each
-  const long long most = kDisBytes / bytes;
-  d.team = int((p->vocab + most - 1) / most);
-  while (d.team < 8 && 2LL * p->rows * d.team <= 148 && p->vocab > d.team * 4096) ++d.team;
-  d.slice = ((p->vocab + d.team - 1) / d.team + 31) & ~31;
   switch (p->dtype) {
-    case DS41_B200_F32: return int(launch_distill<float, kMode, 512>(d, stream));
-    case DS41_B200_BF16: return int(launch_distill<__nv_bfloat16, kMode, 512>(d, stream));
-    default: return int(launch_distill<__half, kMode, 512>(d, stream));
+    case DS41_B200_F32: return int(launch_distill<float, kMode>(d, stream));
+    case DS41_B200_BF16: return int(launch_distill<__nv_bfloat16, kMode>(d, stream));
+    default: return int(launch_distill<__half, kMode>(d, stream));
   }
 }
 

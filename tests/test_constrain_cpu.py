@@ -72,28 +72,34 @@ TEAM_READ = re.compile(r"\bteam_read\(|\bteam_address\(")
 
 
 def test_team_kernels_read_between_barriers():
-    """Another CTA's shared memory is read behind a barrier of the whole team and in front of one (or of the first half of one whose second
-    half ends the kernel), which every thread of every CTA passes that has not left before the first of them."""
+    """Another CTA's shared memory is read behind a barrier of the whole team, and none leaves before a later one."""
     seen = set()
     for name, kernel, _, body in kernels():
-        text = without_lambdas(body)
-        if "team_rank()" not in text:
+        if "team_rank()" not in body:
             assert not TEAM_READ.search(body), (name, kernel)
             continue
         seen.add(kernel)
-        variant = "if constexpr (kTeam) {"        # (a kernel may have a variant without teams)
-        if variant in text:
-            part = braced(text, text.index(variant))
-            assert not TEAM_READ.search(text.replace(part, "")) and "team_barrier" not in text.replace(part, ""), kernel
-            text = part
-        barriers = [m.start() for m in re.finditer(r"\bteam_(?:barrier|arrive|wait)\(\);", text)]
-        assert not any(enclosing(text, b) for b in barriers), kernel
-        kinds = re.findall(r"\bteam_(barrier|arrive|wait)\(", text)
-        assert kinds in (["barrier", "barrier"], ["barrier", "arrive", "wait"]), (kernel, kinds)
-        accesses = [m.start() for m in TEAM_READ.finditer(text)]
-        assert accesses and barriers[0] < accesses[0] and accesses[-1] < barriers[1], kernel
-        assert "return;" not in text[barriers[0]:], kernel
-        assert text[barriers[-1]:].strip() in ("team_barrier();", "team_wait();"), kernel
+        if kernel == "constrain_kernel":          # its variant for few rows: two barriers at the end, the reads between them
+            part = braced(body, body.index("if constexpr (kTeam) {"))
+            assert not TEAM_READ.search(body.replace(part, "")) and "team_barrier" not in body.replace(part, "")
+            barriers = [m.start() for m in re.finditer(r"\bteam_barrier\(\);", part)]
+            reads = [m.start() for m in TEAM_READ.finditer(part)]
+            assert len(barriers) == 2 and not any(enclosing(part, b) for b in barriers)
+            assert barriers[0] < reads[0] and reads[-1] < barriers[1] and part.strip().endswith("team_barrier();")
+        else:                                     # a barrier a turn, of both kinds of warps, and one behind the last turn
+            head = "for (int row = own_team; row < a.rows; row += teams, ++turn) {"
+            loop = braced(body, body.index(head))
+            behind = body[body.index(head) + len(head) + len(loop):]
+            assert behind.strip("}; \n").endswith("if (p.team > 1) team_barrier()") and "return;" not in loop
+            listing = braced(loop, loop.index("if (warp >= kWarps) {"))
+            assert re.findall(r"(if \(p\.team > 1\)) team_(\w+)\(\);", listing) == [("if (p.team > 1)", "arrive"), ("if (p.team > 1)", "wait")]
+            assert listing.strip().startswith("if (p.team > 1) team_arrive();") or listing.index("team_arrive") < listing.index("take_list")
+            computing = loop.replace(listing, "")
+            assert re.findall(r"\bteam_(barrier|arrive|wait)\(", computing) == ["barrier"] and "if (p.team > 1) team_barrier();" in computing
+            assert len(TEAM_READ.findall(body)) == 1 and computing.index("team_barrier();") < TEAM_READ.search(computing).start()
+            # the words that are read are those of the turn's parity: written before the barrier, and again behind the next one
+            assert "s.sums[turn & 1][warp] = " in computing[:computing.index("team_barrier();")]
+            assert "team_read(&s.sums[turn & 1]" in computing
     assert seen == {"constrain_kernel", "distill_kernel"}
     users = {n for n in os.listdir(CSRC) if n.endswith((".cu", ".cuh")) and "team_rank()" in source(n)}
     assert users == {"constrain.cu", "distill.cu", "row_team.cuh"}
