@@ -25,14 +25,16 @@ namespace ds41 {
 namespace {
 
 enum DistillMode { kDistillLoss, kDistillGrad, kDistillBoth };
-constexpr int kDisSteps = 17;                 // vectors of a thread, the last one where a slice does not begin on a vector
-constexpr int kDisGroup = 4;                  // of them, those that are waited for together
+constexpr int kDisGroup = 4;                  // vectors of a thread that are copied, waited for and worked on together
+constexpr int kDisGroups = 5;                 // (the last for the one vector more of a slice that does not begin on a vector)
+constexpr int kDisVectors = kDisGroup * (kDisGroups - 1);
 constexpr int kDisTop = DS41_B200_DISTILL_MAX_TOP;
 constexpr int kDisOwn = kDisTop / 32;         // entries of a lane
 constexpr double kDisMost = 1.01;             // what a list's probabilities may add up to: 1, and the rounding of stored values
 
 struct DistillParams {
   ds41_b200_distill_args a;
+  int in_place;                               // grad is logits
   int slice, team;                            // ids of a CTA (a multiple of 32), CTAs of a row
   float log2e_t;                              // log2(e) / T
 };
@@ -41,7 +43,7 @@ __device__ __forceinline__ void copy16_async(const void *to, const void *from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void copies_wait(int left) {   // (a constant where it is called)
+__device__ __forceinline__ void copies_wait(int left) {
   switch (left) {
     case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
     case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
@@ -87,6 +89,9 @@ struct DistillSlice {
     lead = int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % RowType<T>::kVec);
     vecs = (lead + len + RowType<T>::kVec - 1) / RowType<T>::kVec;
   }
+  __device__ __forceinline__ bool whole(int v, int len) const {
+    return v * RowType<T>::kVec >= lead && (v + 1) * RowType<T>::kVec <= lead + len;
+  }
 };
 
 template <class T, int kMode, int kCompute>
@@ -112,17 +117,14 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
 
   auto row_scale = [&](int row) { return kMode != kDistillLoss && a.row_scale && row < a.rows ? load_input(a.row_scale + row) : 1.f; };
   auto skipped = [&](const DistillRow &r) { return kMode != kDistillLoss && r.scale == 0.f; };
-  auto partial = [&](const DistillSlice<T> &c, int v) { return v * kVec < c.lead || (v + 1) * kVec > c.lead + len; };
   auto start_copy = [&](const DistillSlice<T> &c, int v) {   // a vector that is not whole comes by its ids
     if (v >= c.vecs) return;
-    if (!partial(c, v)) {
+    if (c.whole(v, len)) {
       copy16_async(&stage[v], reinterpret_cast<const uint4 *>(c.x - c.lead) + v);
     } else {
       T *each = reinterpret_cast<T *>(&stage[v]);
-      for (int k = 0; k < kVec; ++k) {
-        const int i = v * kVec + k - c.lead;
-        if (i >= 0 && i < len) each[k] = c.x[i];
-      }
+#pragma unroll 1
+      for (int i = max(0, v * kVec - c.lead); i < min(len, (v + 1) * kVec - c.lead); ++i) each[i + c.lead - v * kVec] = c.x[i];
     }
   };
 
@@ -291,114 +293,112 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
     if (a.stats) reinterpret_cast<float4 *>(a.stats)[row] = stats;
   };
 
-  // ---- the first row on its way
-  if (warp < kWarps) {
-    if (row_scale(own_team) != 0.f) {
-      const DistillSlice<T> c(p, own_team, begin, len);
-#pragma unroll
-      for (int g = 0; g < kDisSteps; ++g) {
-        start_copy(c, tid + g * kCompute);
-        if (g % kDisGroup == kDisGroup - 1 || g == kDisSteps - 1) copies_commit();
-      }
-    }
-  } else if (warp == kWarps) {
-    take_list(own_team, 0);
-  } else {
-    if (lane < 2) s.rows[lane].scale = row_scale(own_team + lane * teams);
-    take_bits(own_team, 0);
-  }
-  __syncthreads();
-
-  int turn = 0;
-  for (int row = own_team; row < a.rows; row += teams, ++turn) {
-    const int next = row + teams;
+  const bool together = p.team > 1 && (kMode != kDistillGrad || p.in_place);   // the team's CTAs wait for one another every turn
+  const int turns = (a.rows - own_team + teams - 1) / teams;
+  for (int turn = -1; turn <= turns; ++turn) {  // (one ahead for the first list and copies, one behind for the last loss)
+    const int row = own_team + turn * teams, next = row + teams;
+    const bool has = turn >= 0 && turn < turns, has_next = turn + 1 < turns;
     if (warp >= kWarps) {                     // a row ahead
-      if (p.team > 1) team_arrive();
+      if (together && has) team_arrive();
       if (warp == kWarps) {
-        if (next < a.rows) take_list(next, turn + 1);
+        if (has_next) take_list(next, turn + 1);
       } else {
         if (lane == 0) s.rows[(turn + 2) & 3].scale = row_scale(next + teams);
-        if (next < a.rows) take_bits(next, turn + 1);
+        if (lane == 0 && turn < 0) s.rows[0].scale = row_scale(next);
+        if (has_next) take_bits(next, turn + 1);
         if (kMode != kDistillGrad && rank == 0 && lane == 0 && turn > 0) finish(row - teams, turn - 1);
       }
-      if (p.team > 1) team_wait();
+      if (together && has) team_wait();
+    } else if (!has) {
+      if (has_next && row_scale(next) != 0.f) {
+        const DistillSlice<T> c(p, next, begin, len);
+#pragma unroll 1
+        for (int g = 0; g < kDisGroups; ++g) {
+#pragma unroll
+          for (int u = 0; u < kDisGroup; ++u) start_copy(c, tid + (g * kDisGroup + u) * kCompute);
+          copies_commit();
+        }
+      }
     } else {
       const DistillRow &r = s.rows[turn & 3];
-      const DistillSlice<T> c(p, row, begin, len), c_next(p, next < a.rows ? next : row, begin, len);
-      const bool skip = skipped(r), ahead = next < a.rows && !skipped(s.rows[(turn + 1) & 3]);
+      const DistillSlice<T> c(p, row, begin, len), c_next(p, has_next ? next : row, begin, len);
+      const bool skip = skipped(r), ahead = has_next && !skipped(s.rows[(turn + 1) & 3]);
       const uint32_t *const in_sum = bits + (turn & 1) * bits_room;
       const float2x c2 = pack_f32x2(p.log2e_t, p.log2e_t);
       T *const grad = kMode == kDistillLoss ? nullptr : static_cast<T *>(a.grad) + size_t(row) * size_t(a.grad_stride) + begin;
       const bool by_vectors = kMode != kDistillLoss && int((reinterpret_cast<uintptr_t>(grad) / sizeof(T)) % kVec) == c.lead;
-      // the vector's ids that are in the sum; the others are -inf
-      auto values = [&](int v, float (&y)[kVec]) {
-        R::unpack(stage[v], y);
-        const unsigned in = (in_sum[v * kVec >> 5] >> (v * kVec & 31)) & kAll;
-        if (in == kAll) return false;
-#pragma unroll
-        for (int k = 0; k < kVec; ++k) y[k] = (in >> k) & 1u ? y[k] : -INFINITY;
-        return true;
-      };
       auto put = [&](int v, const uint4 &q) {
-        if (by_vectors && !partial(c, v)) {
+        if (by_vectors && c.whole(v, len)) {
           reinterpret_cast<uint4 *>(grad - c.lead)[v] = q;
-        } else {
-          const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-          for (int k = 0; k < kVec; ++k) {
-            const int i = v * kVec + k - c.lead;
-            T each;
-            if constexpr (sizeof(T) == 4) each = __uint_as_float(w[k]);
-            else *reinterpret_cast<uint16_t *>(&each) = uint16_t(w[k / 2] >> (k % 2 * 16));
-            if (i >= 0 && i < len) grad[i] = each;
-          }
+        } else {                              // (by way of the stage, where the vector is not needed any more)
+          stage[v] = q;
+          const T *each = reinterpret_cast<const T *>(&stage[v]);
+#pragma unroll 1
+          for (int i = max(0, v * kVec - c.lead); i < min(len, (v + 1) * kVec - c.lead); ++i) grad[i] = each[i + c.lead - v * kVec];
         }
       };
-      // f(v) over the thread's vectors; kArrive: as their copies arrive; kNext: behind each the copy of the next row's
+      // f(vectors, how many of them, first, ...) over the thread's vectors by groups.  arrive: as their copies do; start_next: behind each
+      // group the copies of the next row's, so that as many groups are on their way as before
       auto run = [&](auto arrive, auto start_next, auto f) {
-#pragma unroll
-        for (int g = 0; g < kDisSteps; ++g) {
-          // (with a group of the next row's behind each of this one's, the newest four may always be on their way)
-          if (arrive.value && g % kDisGroup == 0) copies_wait((kDisSteps - 1) / kDisGroup - (start_next.value && ahead ? 0 : g / kDisGroup));
-          const int v = tid + g * kCompute;
-          if (v < c.vecs) f(v);
+#pragma unroll 1
+        for (int g = 0; g < kDisGroups; ++g) {
+          const int v0 = tid + g * kDisGroup * kCompute;
+          if (arrive.value) copies_wait(kDisGroups - 1 - (start_next.value && ahead ? 0 : g));
+          if (v0 < c.vecs) f(v0);
           if (start_next.value && ahead) {
-            start_copy(c_next, v);
-            if (g % kDisGroup == kDisGroup - 1 || g == kDisSteps - 1) copies_commit();
+#pragma unroll
+            for (int u = 0; u < kDisGroup; ++u) start_copy(c_next, v0 + u * kCompute);
+            copies_commit();
           }
         }
       };
       using Yes = std::true_type;
       using No = std::false_type;
+      // a vector; ids that are not in the sum are -inf
+      auto vector = [&](int v, uint4 &q) {
+        q = stage[v];
+        const unsigned in = (in_sum[v * kVec >> 5] >> (v * kVec & 31)) & kAll;
+        if (in == kAll) return false;
+        q = R::only(q, in);
+        return true;
+      };
 
       // ---- maximum and sum of the ids outside the list
       float high = -FLT_MAX;
-      float2x sum2 = pack_f32x2(0.f, 0.f);
-      auto add = [&](int v) {
-        float y[kVec];
-        const bool changed = values(v, y);
-        if (kMode == kDistillBoth && changed) stage[v] = R::pack(y);
-        float top = y[0];
+      float2x sums[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
+      auto add = [&](int v0) {
+        uint4 q[kDisGroup];
 #pragma unroll
-        for (int k = 1; k < kVec; ++k) top = fmaxf(top, y[k]);
+        for (int u = 0; u < kDisGroup; ++u) {
+          const int v = v0 + u * kCompute;
+          q[u] = R::nothing();
+          if (v < c.vecs && vector(v, q[u]) && kMode == kDistillBoth) stage[v] = q[u];
+        }
+        const float top = R::largest(q);
         if (top > high) {
           const float down = exp2_approx((high - top) * p.log2e_t);
-          sum2 = mul_f32x2(sum2, pack_f32x2(down, down));
+          sums[0] = mul_f32x2(sums[0], pack_f32x2(down, down));
+          sums[1] = mul_f32x2(sums[1], pack_f32x2(down, down));
           high = top;
         }
         const float2x minus = pack_f32x2(-high, -high);
 #pragma unroll
-        for (int k = 0; k < kVec; k += 2) {
-          float e0, e1;
-          unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(y[k], y[k + 1]), minus), c2), e0, e1);
-          sum2 = add_f32x2(sum2, pack_f32x2(exp2_approx(e0), exp2_approx(e1)));
+        for (int u = 0; u < kDisGroup; ++u) {
+          float y[kVec];
+          R::unpack(q[u], y);
+#pragma unroll
+          for (int k = 0; k < kVec; k += 2) {
+            float e0, e1;
+            unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(y[k], y[k + 1]), minus), c2), e0, e1);
+            sums[k / 2 % 2] = add_f32x2(sums[k / 2 % 2], pack_f32x2(exp2_approx(e0), exp2_approx(e1)));
+          }
         }
       };
       if (kMode == kDistillLoss) run(Yes{}, Yes{}, add);
       if (kMode == kDistillBoth && !skip) run(Yes{}, No{}, add);
       if (kMode != kDistillGrad) {
         float s0, s1, all = high;
-        unpack_f32x2(sum2, s0, s1);
+        unpack_f32x2(add_f32x2(sums[0], sums[1]), s0, s1);
 #pragma unroll
         for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
         float sum = (s0 + s1) * exp2_approx((high - all) * p.log2e_t);
@@ -406,8 +406,8 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) s.sums[turn & 1][warp] = make_float2(all, sum);
       }
-      if (p.team > 1) team_barrier();         // every CTA has its sums, and has read of the row what it needs of other slices
-      else barrier_of<1, kCompute>();
+      if (together) team_barrier();           // every CTA has its sums, and has read of the row what it needs of other slices
+      else if (kMode != kDistillGrad) barrier_of<1, kCompute>();
       float rest_max = -FLT_MAX, rest_sum = 0.f;
       if (kMode != kDistillGrad) {
         for (int w = lane; w < kWarps * p.team; w += 32) {            // (64 at most: two a lane, of the same order everywhere)
@@ -454,22 +454,36 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
           uint32_t w = 0u;
           if (!skip && reject != DS41_B200_ROW_EMPTY)
             w = sizeof(T) == 4 ? *reinterpret_cast<const uint32_t *>(&nan) : *reinterpret_cast<const uint16_t *>(&nan) * 0x10001u;
-          const uint4 q = make_uint4(w, w, w, w);
           if (!skip) copies_wait(0);
-          run(No{}, Yes{}, [&](int v) { put(v, q); });
+          run(No{}, Yes{}, [&](int v0) {
+#pragma unroll 1
+            for (int v = v0; v < min(c.vecs, v0 + kDisGroup * kCompute); v += kCompute) put(v, make_uint4(w, w, w, w));
+          });
         } else {
           const float2x minus = pack_f32x2(-rest_max, -rest_max), coef2 = pack_f32x2(coef, coef);
-          auto step = [&](int v) {
-            float y[kVec];
-            if (kMode == kDistillGrad) values(v, y);
-            else R::unpack(stage[v], y);
+          auto step = [&](int v0) {
+            uint4 q[kDisGroup];
 #pragma unroll
-            for (int k = 0; k < kVec; k += 2) {
-              float e0, e1;
-              unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(y[k], y[k + 1]), minus), c2), e0, e1);
-              unpack_f32x2(mul_f32x2(pack_f32x2(exp2_approx(e0), exp2_approx(e1)), coef2), y[k], y[k + 1]);
+            for (int u = 0; u < kDisGroup; ++u) {
+              const int v = v0 + u * kCompute;
+              if (v >= c.vecs) continue;
+              if (kMode == kDistillGrad) vector(v, q[u]);
+              else q[u] = stage[v];
             }
-            put(v, R::pack(y));
+#pragma unroll
+            for (int u = 0; u < kDisGroup; ++u) {
+              const int v = v0 + u * kCompute;
+              if (v >= c.vecs) break;
+              float y[kVec];
+              R::unpack(q[u], y);
+#pragma unroll
+              for (int k = 0; k < kVec; k += 2) {
+                float e0, e1;
+                unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(y[k], y[k + 1]), minus), c2), e0, e1);
+                unpack_f32x2(mul_f32x2(pack_f32x2(exp2_approx(e0), exp2_approx(e1)), coef2), y[k], y[k + 1]);
+              }
+              put(v, R::pack(y));
+            }
           };
           if (kMode == kDistillGrad) run(Yes{}, Yes{}, step);
           else run(No{}, Yes{}, step);
@@ -485,7 +499,6 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
     }
     __syncthreads();
   }
-  if (kMode != kDistillGrad && rank == 0 && tid == kCompute + 32) finish(own_team + (turn - 1) * teams, turn - 1);
   if (p.team > 1) team_barrier();
 }
 
@@ -537,7 +550,7 @@ cudaError_t launch_distill(const DistillParams &p, cudaStream_t stream) {
 
 template <class T, int kMode>
 cudaError_t launch_distill(DistillParams &d, cudaStream_t stream) {
-  constexpr int kSmall = 64 * (kDisSteps - 1) * 16 / int(sizeof(T)), kLarge = 4 * kSmall;   // ids of a CTA
+  constexpr int kSmall = 64 * kDisVectors * 16 / int(sizeof(T)), kLarge = 4 * kSmall;   // ids of a CTA
   const int vocab = d.a.vocab, top = d.a.top;
   // CTAs per row: as few as hold it, three CTAs to an SM where eight of them can, and for batches that leave SMs idle up to eight, of at least
   // 4096 ids each
@@ -577,7 +590,7 @@ int distill(const ds41_b200_distill_args *p, cudaStream_t stream) {
     if (!rows_apart_or_same(p->logits, p->logits_stride, p->grad, p->grad_stride, p->rows, p->vocab, bytes))
       return invalid("distill args: grad overlaps logits without being the same rows");
   }
-  DistillParams d{*p, 0, 1, float(1.4426950408889634 / p->temperature)};
+  DistillParams d{*p, p->grad == p->logits, 0, 1, float(1.4426950408889634 / p->temperature)};
   switch (p->dtype) {
     case DS41_B200_F32: return int(launch_distill<float, kMode>(d, stream));
     case DS41_B200_BF16: return int(launch_distill<__nv_bfloat16, kMode>(d, stream));

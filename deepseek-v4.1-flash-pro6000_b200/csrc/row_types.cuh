@@ -20,6 +20,20 @@ template <> struct RowType<float> {
     return fmaf(__uint_as_float(q.x), 0.f, fmaf(__uint_as_float(q.y), 0.f, fmaf(__uint_as_float(q.z), 0.f, fmaf(__uint_as_float(q.w), 0.f, f))));
   }
   static __device__ __forceinline__ bool all_finite(Finite f) { return f == 0.f; }
+  // -inf everywhere; q where `in` has a bit, -inf elsewhere; the largest of the vectors' values (NaN passed over)
+  static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+  static __device__ __forceinline__ uint4 only(const uint4 &q, unsigned in) {
+    return make_uint4(in & 1u ? q.x : 0xff800000u, in & 2u ? q.y : 0xff800000u, in & 4u ? q.z : 0xff800000u, in & 8u ? q.w : 0xff800000u);
+  }
+  template <int kCount> static __device__ __forceinline__ float largest(const uint4 (&q)[kCount]) {
+    float m[2] = {__uint_as_float(q[0].x), __uint_as_float(q[0].y)};
+#pragma unroll
+    for (int u = 0; u < kCount; ++u) {
+      m[0] = fmaxf(m[0], fmaxf(__uint_as_float(q[u].x), __uint_as_float(q[u].y)));
+      m[1] = fmaxf(m[1], fmaxf(__uint_as_float(q[u].z), __uint_as_float(q[u].w)));
+    }
+    return fmaxf(m[0], m[1]);
+  }
   static __device__ __forceinline__ void unpack(const uint4 &q, float (&x)[4]) {
     x[0] = __uint_as_float(q.x); x[1] = __uint_as_float(q.y); x[2] = __uint_as_float(q.z); x[3] = __uint_as_float(q.w);
   }
@@ -44,6 +58,24 @@ template <> struct RowType<__nv_bfloat16> {
     return f;
   }
   static __device__ __forceinline__ bool all_finite(Finite f) { return __low2float(f) == 0.f && __high2float(f) == 0.f; }
+  static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+  static __device__ __forceinline__ uint4 only(const uint4 &q, unsigned in) {
+    uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t keep = ((in >> 2 * k) & 1u) * 0xffffu | ((in >> (2 * k + 1)) & 1u) * 0xffff0000u;
+      w[k] = (w[k] & keep) | (0xff80ff80u & ~keep);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  template <int kCount> static __device__ __forceinline__ float largest(const uint4 (&q)[kCount]) {
+    const Finite *v = reinterpret_cast<const Finite *>(q);
+    Finite m[2] = {v[0], v[1]};
+#pragma unroll
+    for (int i = 2; i < 4 * kCount; ++i) m[i & 1] = __hmax2(m[i & 1], v[i]);
+    m[0] = __hmax2(m[0], m[1]);
+    return fmaxf(__low2float(m[0]), __high2float(m[0]));
+  }
   static __device__ __forceinline__ void unpack(const uint4 &q, float (&x)[8]) {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -73,6 +105,24 @@ template <> struct RowType<__half> {
     return f;
   }
   static __device__ __forceinline__ bool all_finite(Finite f) { return __low2float(f) == 0.f && __high2float(f) == 0.f; }
+  static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+  static __device__ __forceinline__ uint4 only(const uint4 &q, unsigned in) {
+    uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t keep = ((in >> 2 * k) & 1u) * 0xffffu | ((in >> (2 * k + 1)) & 1u) * 0xffff0000u;
+      w[k] = (w[k] & keep) | (0xfc00fc00u & ~keep);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  template <int kCount> static __device__ __forceinline__ float largest(const uint4 (&q)[kCount]) {
+    const Finite *v = reinterpret_cast<const Finite *>(q);
+    Finite m[2] = {v[0], v[1]};
+#pragma unroll
+    for (int i = 2; i < 4 * kCount; ++i) m[i & 1] = __hmax2(m[i & 1], v[i]);
+    m[0] = __hmax2(m[0], m[1]);
+    return fmaxf(__low2float(m[0]), __high2float(m[0]));
+  }
   static __device__ __forceinline__ void unpack(const uint4 &q, float (&x)[8]) {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll

@@ -87,15 +87,18 @@ def test_team_kernels_read_between_barriers():
             assert len(barriers) == 2 and not any(enclosing(part, b) for b in barriers)
             assert barriers[0] < reads[0] and reads[-1] < barriers[1] and part.strip().endswith("team_barrier();")
         else:                                     # a barrier a turn, of both kinds of warps, and one behind the last turn
-            head = "for (int row = own_team; row < a.rows; row += teams, ++turn) {"
+            head = "for (int turn = -1; turn <= turns; ++turn) {"
             loop = braced(body, body.index(head))
             behind = body[body.index(head) + len(head) + len(loop):]
-            assert behind.strip("}; \n").endswith("if (p.team > 1) team_barrier()") and "return;" not in loop
+            assert behind.strip("}; \n").endswith("if (p.team > 1) team_barrier()") and not re.search(r"\b(?:return|break|continue);", without_lambdas(
+                loop.replace(braced(loop, loop.index("for (int e = tid; e < a.top")), "")))
             listing = braced(loop, loop.index("if (warp >= kWarps) {"))
-            assert re.findall(r"(if \(p\.team > 1\)) team_(\w+)\(\);", listing) == [("if (p.team > 1)", "arrive"), ("if (p.team > 1)", "wait")]
-            assert listing.strip().startswith("if (p.team > 1) team_arrive();") or listing.index("team_arrive") < listing.index("take_list")
-            computing = loop.replace(listing, "")
-            assert re.findall(r"\bteam_(barrier|arrive|wait)\(", computing) == ["barrier"] and "if (p.team > 1) team_barrier();" in computing
+            assert re.findall(r"(if \([^)]*\)) team_(\w+)\(\);", listing) == [("if (together && has)", "arrive"), ("if (together && has)", "wait")]
+            assert listing.index("team_arrive") < listing.index("take_list") < listing.index("team_wait")
+            computing = loop.replace(listing, "")   # (its branch is the one with `has`)
+            assert "} else if (!has) {" in computing
+            assert re.findall(r"\bteam_(barrier|arrive|wait)\(", computing) == ["barrier"] and "if (together) team_barrier();" in computing
+            assert "const bool together = p.team > 1 && (kMode != kDistillGrad || p.in_place);" in body
             assert len(TEAM_READ.findall(body)) == 1 and computing.index("team_barrier();") < TEAM_READ.search(computing).start()
             # the words that are read are those of the turn's parity: written before the barrier, and again behind the next one
             assert "s.sums[turn & 1][warp] = " in computing[:computing.index("team_barrier();")]
