@@ -63,6 +63,11 @@ __device__ __forceinline__ float exp2_approx(float x) {   // 2 ulp; 0 for -inf a
   return y;
 }
 
+// Out of line, once each: what runs a few times a row shall not push the loops out of the instruction cache.
+__device__ __noinline__ double exp_of(double x) { return exp(x); }
+__device__ __noinline__ double log_of(double x) { return log(x); }
+__device__ __noinline__ double over(double x, double y) { return x / y; }
+
 // What is known of a row besides its ids outside the list, the same in every CTA of the team.
 struct DistillRow {
   float scale;
@@ -94,6 +99,13 @@ struct DistillSlice {
   }
 };
 
+// A vector that is not whole comes and goes by its ids, `from` .. `to`.
+template <class T>
+__device__ __noinline__ void copy_ids(T *to_first, const T *from_first, int from, int to) {
+#pragma unroll 1
+  for (int i = from; i < to; ++i) to_first[i] = from_first[i];
+}
+
 template <class T, int kMode, int kCompute>
 __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distill_kernel(DistillParams p) {
   using R = RowType<T>;
@@ -117,15 +129,15 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
 
   auto row_scale = [&](int row) { return kMode != kDistillLoss && a.row_scale && row < a.rows ? load_input(a.row_scale + row) : 1.f; };
   auto skipped = [&](const DistillRow &r) { return kMode != kDistillLoss && r.scale == 0.f; };
-  auto start_copy = [&](const DistillSlice<T> &c, int v) {   // a vector that is not whole comes by its ids
-    if (v >= c.vecs) return;
-    if (c.whole(v, len)) {
-      copy16_async(&stage[v], reinterpret_cast<const uint4 *>(c.x - c.lead) + v);
-    } else {
-      T *each = reinterpret_cast<T *>(&stage[v]);
-#pragma unroll 1
-      for (int i = max(0, v * kVec - c.lead); i < min(len, (v + 1) * kVec - c.lead); ++i) each[i + c.lead - v * kVec] = c.x[i];
+  // the copies of a group of the thread's vectors, from v0 on
+  auto start_copies = [&](const DistillSlice<T> &c, int v0) {
+#pragma unroll
+    for (int u = 0; u < kDisGroup; ++u) {
+      const int v = v0 + u * kCompute;
+      if (c.whole(v, len)) copy16_async(&stage[v], reinterpret_cast<const uint4 *>(c.x - c.lead) + v);
+      else if (v < c.vecs) copy_ids<T>(reinterpret_cast<T *>(stage) + c.lead, c.x, max(0, v * kVec - c.lead), min(len, (v + 1) * kVec - c.lead));
     }
+    copies_commit();
   };
 
   // ---- the list of the row of turn `turn`, by one warp
@@ -140,6 +152,7 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
     unsigned named = 0u, counts = 0u;         // a bit per entry of the lane
     bool bad = false;
     float most = -FLT_MAX, zmax = -FLT_MAX;
+#pragma unroll 1
     for (int k = 0; k < own; ++k) {
       const int e = lane + 32 * k;
       int id = -1;
@@ -169,9 +182,11 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
     }
     __syncwarp();
     unsigned first = counts;                  // entries with no other of the same id in front of them
+#pragma unroll 1
     for (int k = 0; k < own; ++k) {
       if (!((counts >> k) & 1u)) continue;
       const int e = lane + 32 * k, id = id_list[e];
+#pragma unroll 2
       for (int j = 0; 4 * j < e; ++j) {
         const int4 q = reinterpret_cast<const int4 *>(id_list)[j];
         const int before = e - 4 * j;
@@ -181,17 +196,18 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
     const bool again = __any_sync(0xffffffffu, first != counts);
     double list = 0.0, kept = 0.0, entropy = 0.0;
     float share = 0.f;
+#pragma unroll 1
     for (int k = 0; k < own; ++k) {
       const int e = lane + 32 * k;
       if (!((named >> k) & 1u)) continue;
-      const double log_w = a.tail ? w_list[e] : (w_list[e] - double(most)) / t, w = exp(log_w);
+      const double log_w = a.tail ? w_list[e] : over(w_list[e] - double(most), t), w = exp_of(log_w);
       list += w;
       const bool is = (counts >> k) & 1u;
       w_list[e] = is ? w : 0.0;
       if (!is) continue;
       kept += w;
       if (!again) {
-        const double gap = (double(z_list[e]) - double(zmax)) / t;
+        const double gap = over(double(z_list[e]) - double(zmax), t);
         if (w > 0.0) entropy += w * (log_w - gap);
         share += exp2_approx((z_list[e] - zmax) * p.log2e_t);
       }
@@ -199,18 +215,21 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
     if (again) {                              // an id's first entry takes the weights of the later ones
       __syncwarp();
       double merged[kDisOwn];
-      for (int k = 0; k < own; ++k) {
+#pragma unroll 1
+    for (int k = 0; k < own; ++k) {
         const int e = lane + 32 * k;
         merged[k] = e < a.top ? w_list[e] : 0.0;
         if (!((first >> k) & 1u)) continue;
+#pragma unroll 1
         for (int j = e + 1; j < a.top; ++j)
           if (id_list[j] == id_list[e]) merged[k] += w_list[j];
-        const double gap = (double(z_list[e]) - double(zmax)) / t;
-        if (merged[k] > 0.0) entropy += merged[k] * (log(merged[k]) - gap);
+        const double gap = over(double(z_list[e]) - double(zmax), t);
+        if (merged[k] > 0.0) entropy += merged[k] * (log_of(merged[k]) - gap);
         share += exp2_approx((z_list[e] - zmax) * p.log2e_t);
       }
       __syncwarp();
-      for (int k = 0; k < own; ++k) {
+#pragma unroll 1
+    for (int k = 0; k < own; ++k) {
         const int e = lane + 32 * k;
         if (e >= a.top) continue;
         w_list[e] = merged[k];
@@ -229,12 +248,13 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
       r.reject = bad ? DS41_B200_ROW_NONFINITE : a.tail && list > kDisMost ? DS41_B200_ROW_NOT_NORMALIZED : !(kept > 0.0) ? DS41_B200_ROW_EMPTY : 0;
       r.zmax = zmax; r.share = share; r.kept = kept; r.entropy = entropy;
       r.rest = a.tail ? fmax(0.0, 1.0 - list) : 0.0;
-      r.inverse = 1.0 / kept; r.inverse_rest = 1.0 / (kept + r.rest);
+      r.inverse = over(1.0, kept); r.inverse_rest = over(1.0, kept + r.rest);
       if (kMode == kDistillGrad) r.stats = reinterpret_cast<const float4 *>(a.stats)[row];
     }
     barrier_of<2, 64>();                      // (the bits are set)
     const DistillSlice<T> c(p, row, begin, len);
     uint32_t *const out = bits + (turn & 1) * bits_room;
+#pragma unroll 1
     for (int k = 0; k < own; ++k) {
       const int e = lane + 32 * k;
       const unsigned local = e < a.top ? unsigned(id_list[e]) - unsigned(begin) : ~0u;
@@ -249,19 +269,23 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
     const DistillSlice<T> c(p, row, begin, len);
     uint32_t *const out = bits + (turn & 1) * bits_room;
     const uint32_t *mask = a.mask ? a.mask + size_t(row) * size_t(a.mask_stride) : nullptr;
-    const int first = begin / 32, words = (a.vocab + 31) / 32;
-    auto word = [&](int at) { return at >= 0 && at < words ? load_input(mask + at) : 0u; };
-#pragma unroll 8
-    for (int w = lane; w <= (c.lead + len) / 32; w += 32) {
-      uint32_t in = ~0u;
-      if (mask) {
-        in = word(first + w);
-        if (c.lead) in = in << c.lead | word(first + w - 1) >> (32 - c.lead);
+    const int words = (a.vocab + 31) / 32 - begin / 32, last = (c.lead + len) / 32;
+    if (mask) {
+      const uint32_t *from = mask + begin / 32;
+#pragma unroll 4
+      for (int w = lane; w <= last; w += 32) {
+        uint32_t in = w < words ? load_input(from + w) : 0u;
+        if (c.lead) in = in << c.lead | (w > 0 ? load_input(from + w - 1) >> (32 - c.lead) : 0u);
+        out[w] = in;
       }
-      const int low = c.lead - 32 * w, high = c.lead + len - 32 * w;  // of the slice's places
-      if (low > 0) in &= low < 32 ? ~0u << low : 0u;
-      if (high < 32) in &= high > 0 ? (1u << high) - 1u : 0u;
-      out[w] = in;
+    } else {
+#pragma unroll 4
+      for (int w = lane; w <= last; w += 32) out[w] = ~0u;
+    }
+    __syncwarp();
+    if (lane == 0) {                          // nothing in front of the slice's first place or behind its last
+      out[0] &= ~0u << c.lead;
+      out[last] &= (1u << ((c.lead + len) & 31)) - 1u;
     }
     barrier_of<2, 64>();
   };
@@ -280,11 +304,12 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
     if (!reject) {
       const bool any = rest_sum != 0.f;
       const double zmax = r.zmax, largest = any ? fmax(double(rest_max), zmax) : zmax;
-      const double log_rest = log(double(rest_sum));
-      const double log_sum = log((any ? double(rest_sum) * exp((double(rest_max) - largest) / t) : 0.0) + double(r.share) * exp((zmax - largest) / t));
+      const double down = any ? over(double(rest_max) - largest, t) : 0.0, list_down = over(zmax - largest, t);
+      const double log_rest = log_of(double(rest_sum));
+      const double log_sum = log_of((any ? double(rest_sum) * exp_of(down) : 0.0) + double(r.share) * exp_of(list_down));
       const double inverse = any ? r.inverse_rest : r.inverse, kept = r.kept * inverse, tail = any ? r.rest * inverse : 0.0;
-      double sum = r.entropy * inverse + kept * (log(inverse) + log_sum - (zmax - largest) / t);
-      if (tail > 0.0) sum += tail * (log(tail) - ((double(rest_max) - largest) / t + log_rest - log_sum));
+      double sum = r.entropy * inverse + kept * (log_of(inverse) + log_sum - list_down);
+      if (tail > 0.0) sum += tail * (log_of(tail) - (down + log_rest - log_sum));
       loss = float(t * t * sum);
       stats = make_float4(float(largest), float(log_sum), any ? rest_max : -INFINITY, any ? float(log_rest) : -INFINITY);
     }
@@ -313,11 +338,7 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
       if (has_next && row_scale(next) != 0.f) {
         const DistillSlice<T> c(p, next, begin, len);
 #pragma unroll 1
-        for (int g = 0; g < kDisGroups; ++g) {
-#pragma unroll
-          for (int u = 0; u < kDisGroup; ++u) start_copy(c, tid + (g * kDisGroup + u) * kCompute);
-          copies_commit();
-        }
+        for (int g = 0; g < kDisGroups; ++g) start_copies(c, tid + g * kDisGroup * kCompute);
       }
     } else {
       const DistillRow &r = s.rows[turn & 3];
@@ -332,12 +353,10 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
           reinterpret_cast<uint4 *>(grad - c.lead)[v] = q;
         } else {                              // (by way of the stage, where the vector is not needed any more)
           stage[v] = q;
-          const T *each = reinterpret_cast<const T *>(&stage[v]);
-#pragma unroll 1
-          for (int i = max(0, v * kVec - c.lead); i < min(len, (v + 1) * kVec - c.lead); ++i) grad[i] = each[i + c.lead - v * kVec];
+          copy_ids<T>(grad, reinterpret_cast<const T *>(stage) + c.lead, max(0, v * kVec - c.lead), min(len, (v + 1) * kVec - c.lead));
         }
       };
-      // f(vectors, how many of them, first, ...) over the thread's vectors by groups.  arrive: as their copies do; start_next: behind each
+      // f(first vector) over the thread's vectors by groups.  arrive: as their copies do; start_next: behind each
       // group the copies of the next row's, so that as many groups are on their way as before
       auto run = [&](auto arrive, auto start_next, auto f) {
 #pragma unroll 1
@@ -345,11 +364,7 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
           const int v0 = tid + g * kDisGroup * kCompute;
           if (arrive.value) copies_wait(kDisGroups - 1 - (start_next.value && ahead ? 0 : g));
           if (v0 < c.vecs) f(v0);
-          if (start_next.value && ahead) {
-#pragma unroll
-            for (int u = 0; u < kDisGroup; ++u) start_copy(c_next, v0 + u * kCompute);
-            copies_commit();
-          }
+          if (start_next.value && ahead) start_copies(c_next, v0);
         }
       };
       using Yes = std::true_type;
@@ -449,44 +464,38 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
         const double inverse = any ? r.inverse_rest : r.inverse;
         const double factor = double(r.scale) * t;
         const float tail = any ? float(r.rest * inverse) : 0.f, coef = any ? float(factor) * (q_rest - tail) / rest_sum : 0.f;
-        if (skip || reject) {
-          const T nan = R::store(__int_as_float(0x7fffffff));
-          uint32_t w = 0u;
-          if (!skip && reject != DS41_B200_ROW_EMPTY)
-            w = sizeof(T) == 4 ? *reinterpret_cast<const uint32_t *>(&nan) : *reinterpret_cast<const uint16_t *>(&nan) * 0x10001u;
-          if (!skip) copies_wait(0);
-          run(No{}, Yes{}, [&](int v0) {
-#pragma unroll 1
-            for (int v = v0; v < min(c.vecs, v0 + kDisGroup * kCompute); v += kCompute) put(v, make_uint4(w, w, w, w));
-          });
-        } else {
-          const float2x minus = pack_f32x2(-rest_max, -rest_max), coef2 = pack_f32x2(coef, coef);
-          auto step = [&](int v0) {
-            uint4 q[kDisGroup];
+        const bool fill = skip || reject != 0;
+        const T nan = R::store(__int_as_float(0x7fffffff));
+        uint32_t filling = 0u;
+        if (!skip && reject != DS41_B200_ROW_EMPTY)
+          filling = sizeof(T) == 4 ? *reinterpret_cast<const uint32_t *>(&nan) : *reinterpret_cast<const uint16_t *>(&nan) * 0x10001u;
+        const float2x minus = pack_f32x2(-rest_max, -rest_max), coef2 = pack_f32x2(coef, coef);
+        auto step = [&](int v0) {
+          uint4 q[kDisGroup];
 #pragma unroll
-            for (int u = 0; u < kDisGroup; ++u) {
-              const int v = v0 + u * kCompute;
-              if (v >= c.vecs) continue;
-              if (kMode == kDistillGrad) vector(v, q[u]);
-              else q[u] = stage[v];
+          for (int u = 0; u < kDisGroup; ++u) {
+            const int v = v0 + u * kCompute;
+            if (v >= c.vecs) continue;
+            if (kMode == kDistillGrad) vector(v, q[u]);
+            else q[u] = stage[v];
+          }
+#pragma unroll
+          for (int u = 0; u < kDisGroup; ++u) {
+            const int v = v0 + u * kCompute;
+            if (v >= c.vecs) break;
+            float y[kVec];
+            R::unpack(q[u], y);
+#pragma unroll
+            for (int k = 0; k < kVec; k += 2) {
+              float e0, e1;
+              unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(y[k], y[k + 1]), minus), c2), e0, e1);
+              unpack_f32x2(mul_f32x2(pack_f32x2(exp2_approx(e0), exp2_approx(e1)), coef2), y[k], y[k + 1]);
             }
-#pragma unroll
-            for (int u = 0; u < kDisGroup; ++u) {
-              const int v = v0 + u * kCompute;
-              if (v >= c.vecs) break;
-              float y[kVec];
-              R::unpack(q[u], y);
-#pragma unroll
-              for (int k = 0; k < kVec; k += 2) {
-                float e0, e1;
-                unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(y[k], y[k + 1]), minus), c2), e0, e1);
-                unpack_f32x2(mul_f32x2(pack_f32x2(exp2_approx(e0), exp2_approx(e1)), coef2), y[k], y[k + 1]);
-              }
-              put(v, R::pack(y));
-            }
-          };
-          if (kMode == kDistillGrad) run(Yes{}, Yes{}, step);
-          else run(No{}, Yes{}, step);
+            put(v, fill ? make_uint4(filling, filling, filling, filling) : R::pack(y));
+          }
+        };
+        run(std::integral_constant<bool, kMode == kDistillGrad>{}, Yes{}, step);
+        if (!fill) {
           barrier_of<1, kCompute>();          // (zeros stand where listed ids are)
           for (int e = tid; e < a.top; e += kCompute) {
             const unsigned local = unsigned(ids[(turn & 1) * top_room + e]) - unsigned(begin);
