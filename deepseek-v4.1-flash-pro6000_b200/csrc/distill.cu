@@ -88,15 +88,16 @@ struct DistillSmem {
 template <class T>
 struct DistillSlice {
   const T *x;
-  int lead, vecs;
+  int lead, vecs, first_whole, wholes;        // vectors; those of which no id is another slice's
   __device__ __forceinline__ DistillSlice(const DistillParams &p, int row, int begin, int len) {
+    constexpr int kVec = RowType<T>::kVec;
     x = static_cast<const T *>(p.a.logits) + size_t(row) * size_t(p.a.logits_stride) + begin;
-    lead = int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % RowType<T>::kVec);
-    vecs = (lead + len + RowType<T>::kVec - 1) / RowType<T>::kVec;
+    lead = int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % kVec);
+    vecs = (lead + len + kVec - 1) / kVec;
+    first_whole = lead ? 1 : 0;
+    wholes = max(0, (lead + len) / kVec - first_whole);
   }
-  __device__ __forceinline__ bool whole(int v, int len) const {
-    return v * RowType<T>::kVec >= lead && (v + 1) * RowType<T>::kVec <= lead + len;
-  }
+  __device__ __forceinline__ bool whole(int v) const { return unsigned(v - first_whole) < unsigned(wholes); }
 };
 
 // A vector that is not whole comes and goes by its ids, `from` .. `to`.
@@ -104,6 +105,11 @@ template <class T>
 __device__ __noinline__ void copy_ids(T *to_first, const T *from_first, int from, int to) {
 #pragma unroll 1
   for (int i = from; i < to; ++i) to_first[i] = from_first[i];
+}
+
+// Words of bits for a slice of so many bytes.
+template <int kCompute> __host__ __device__ __forceinline__ int distill_bit_words(int bytes) {
+  return (bytes / 16 + 1 + kDisGroup * kCompute - 1) / (kDisGroup * kCompute) * kCompute;
 }
 
 template <class T, int kMode, int kCompute>
@@ -117,12 +123,16 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = int(team_rank()), teams = int(gridDim.x) / p.team, own_team = int(blockIdx.x) / p.team;
   const int begin = min(a.vocab, rank * p.slice), len = min(a.vocab - begin, p.slice);
-  const int top_room = (a.top + 3) & ~3, bits_room = p.slice / 32 + 2;
+  const int top_room = (a.top + 3) & ~3, bits_room = distill_bit_words<kCompute>(p.slice * int(sizeof(T)));
   uint4 *const behind = stage + p.slice * int(sizeof(T)) / 16 + 1;
   double *const weights = reinterpret_cast<double *>(behind);
   int *const ids = reinterpret_cast<int *>(weights + 2 * top_room);
   float *const zs = reinterpret_cast<float *>(ids + 2 * top_room);
-  uint32_t *const bits = reinterpret_cast<uint32_t *>(zs + 2 * top_room);   // by place: allowed and not listed
+  // which ids are in the sum (allowed and not listed): a word holds the bits of the four vectors that a thread takes together
+  uint32_t *const bits = reinterpret_cast<uint32_t *>(zs + 2 * top_room);
+  uint32_t *const mask_words = bits + 2 * bits_room;   // of the slice, as they come
+  auto bit_word = [](int v) { return v / (kDisGroup * kCompute) * kCompute + v % kCompute; };
+  auto bit_shift = [](int v) { return v / kCompute % kDisGroup * kVec; };
   const double t = a.temperature;
   cudaGridDependencySynchronize();
   cudaTriggerProgrammaticLaunchCompletion();
@@ -134,7 +144,7 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
 #pragma unroll
     for (int u = 0; u < kDisGroup; ++u) {
       const int v = v0 + u * kCompute;
-      if (c.whole(v, len)) copy16_async(&stage[v], reinterpret_cast<const uint4 *>(c.x - c.lead) + v);
+      if (c.whole(v)) copy16_async(&stage[v], reinterpret_cast<const uint4 *>(c.x - c.lead) + v);
       else if (v < c.vecs) copy_ids<T>(reinterpret_cast<T *>(stage) + c.lead, c.x, max(0, v * kVec - c.lead), min(len, (v + 1) * kVec - c.lead));
     }
     copies_commit();
@@ -259,8 +269,8 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
       const int e = lane + 32 * k;
       const unsigned local = e < a.top ? unsigned(id_list[e]) - unsigned(begin) : ~0u;
       if (local < unsigned(len)) {
-        const unsigned place = local + unsigned(c.lead);
-        atomicAnd(&out[place >> 5], ~(1u << (place & 31u)));
+        const int place = int(local) + c.lead, v = place / kVec;
+        atomicAnd(&out[bit_word(v)], ~(1u << (bit_shift(v) + place % kVec)));
       }
     }
   };
@@ -268,24 +278,37 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
   auto take_bits = [&](int row, int turn) {
     const DistillSlice<T> c(p, row, begin, len);
     uint32_t *const out = bits + (turn & 1) * bits_room;
-    const uint32_t *mask = a.mask ? a.mask + size_t(row) * size_t(a.mask_stride) : nullptr;
-    const int words = (a.vocab + 31) / 32 - begin / 32, last = (c.lead + len) / 32;
-    if (mask) {
-      const uint32_t *from = mask + begin / 32;
+    if (a.mask) {
+      const uint32_t *from = a.mask + size_t(row) * size_t(a.mask_stride) + begin / 32;
+      const int words = min(p.slice / 32, (a.vocab + 31) / 32 - begin / 32);
 #pragma unroll 4
-      for (int w = lane; w <= last; w += 32) {
-        uint32_t in = w < words ? load_input(from + w) : 0u;
-        if (c.lead) in = in << c.lead | (w > 0 ? load_input(from + w - 1) >> (32 - c.lead) : 0u);
+      for (int w = lane; w < words; w += 32)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(uint32_t(__cvta_generic_to_shared(mask_words + w))), "l"(from + w) : "memory");
+      copies_commit();
+      copies_wait(0);
+      __syncwarp();
+#pragma unroll 1
+      for (int w = lane; w < bits_room; w += 32) {
+        uint32_t in = 0u;
+#pragma unroll
+        for (int u = 0; u < kDisGroup; ++u) {
+          const int v = w / kCompute * kDisGroup * kCompute + u * kCompute + w % kCompute;
+          if (v >= c.vecs) continue;
+          const int at = v * kVec - c.lead, low = max(at, 0);          // (the vector's first id; what is in front of the slice is cut off below)
+          uint32_t some = mask_words[low >> 5] >> (low & 31);
+          if ((low & 31) + kVec > 32 && (low >> 5) + 1 < words) some |= mask_words[(low >> 5) + 1] << (32 - (low & 31));
+          in |= ((some << (low - at)) & kAll) << (u * kVec);
+        }
         out[w] = in;
       }
     } else {
-#pragma unroll 4
-      for (int w = lane; w <= last; w += 32) out[w] = ~0u;
+      for (int w = lane; w < bits_room / 4; w += 32) reinterpret_cast<uint4 *>(out)[w] = make_uint4(~0u, ~0u, ~0u, ~0u);
     }
     __syncwarp();
     if (lane == 0) {                          // nothing in front of the slice's first place or behind its last
-      out[0] &= ~0u << c.lead;
-      out[last] &= (1u << ((c.lead + len) & 31)) - 1u;
+      out[0] &= ~((1u << c.lead) - 1u);
+      const int behind = c.vecs * kVec - c.lead - len, v = c.vecs - 1;
+      if (behind > 0) out[bit_word(v)] &= ~(((1u << behind) - 1u) << (bit_shift(v) + kVec - behind));
     }
     barrier_of<2, 64>();
   };
@@ -344,12 +367,12 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
       const DistillRow &r = s.rows[turn & 3];
       const DistillSlice<T> c(p, row, begin, len), c_next(p, has_next ? next : row, begin, len);
       const bool skip = skipped(r), ahead = has_next && !skipped(s.rows[(turn + 1) & 3]);
-      const uint32_t *const in_sum = bits + (turn & 1) * bits_room;
+      const uint32_t *const in_sum = bits + (turn & 1) * bits_room + tid;
       const float2x c2 = pack_f32x2(p.log2e_t, p.log2e_t);
       T *const grad = kMode == kDistillLoss ? nullptr : static_cast<T *>(a.grad) + size_t(row) * size_t(a.grad_stride) + begin;
       const bool by_vectors = kMode != kDistillLoss && int((reinterpret_cast<uintptr_t>(grad) / sizeof(T)) % kVec) == c.lead;
       auto put = [&](int v, const uint4 &q) {
-        if (by_vectors && c.whole(v, len)) {
+        if (by_vectors && c.whole(v)) {
           reinterpret_cast<uint4 *>(grad - c.lead)[v] = q;
         } else {                              // (by way of the stage, where the vector is not needed any more)
           stage[v] = q;
@@ -369,13 +392,22 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
       };
       using Yes = std::true_type;
       using No = std::false_type;
-      // a vector; ids that are not in the sum are -inf
-      auto vector = [&](int v, uint4 &q) {
-        q = stage[v];
-        const unsigned in = (in_sum[v * kVec >> 5] >> (v * kVec & 31)) & kAll;
-        if (in == kAll) return false;
-        q = R::only(q, in);
-        return true;
+      // a group of vectors; ids that are not in the sum are -inf.  kKeep: in the stage too
+      auto take = [&](int v0, auto keep, uint4 (&q)[kDisGroup]) {
+        uint32_t in = in_sum[(v0 - tid) / kDisGroup];
+#pragma unroll
+        for (int u = 0; u < kDisGroup; ++u) {
+          q[u] = R::nothing();
+          if (v0 + u * kCompute < c.vecs) q[u] = stage[v0 + u * kCompute];
+        }
+        if (sizeof(T) == 4) in |= 0xffff0000u;
+        if (in != ~0u) {
+#pragma unroll
+          for (int u = 0; u < kDisGroup; ++u) {
+            q[u] = R::only(q[u], in >> (u * kVec));
+            if (keep.value && v0 + u * kCompute < c.vecs) stage[v0 + u * kCompute] = q[u];
+          }
+        }
       };
 
       // ---- maximum and sum of the ids outside the list
@@ -383,12 +415,7 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
       float2x sums[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
       auto add = [&](int v0) {
         uint4 q[kDisGroup];
-#pragma unroll
-        for (int u = 0; u < kDisGroup; ++u) {
-          const int v = v0 + u * kCompute;
-          q[u] = R::nothing();
-          if (v < c.vecs && vector(v, q[u]) && kMode == kDistillBoth) stage[v] = q[u];
-        }
+        take(v0, std::integral_constant<bool, kMode == kDistillBoth>{}, q);
         const float top = R::largest(q);
         if (top > high) {
           const float down = exp2_approx((high - top) * p.log2e_t);
@@ -472,12 +499,12 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
         const float2x minus = pack_f32x2(-rest_max, -rest_max), coef2 = pack_f32x2(coef, coef);
         auto step = [&](int v0) {
           uint4 q[kDisGroup];
+          if (kMode == kDistillGrad) {
+            take(v0, No{}, q);
+          } else {
 #pragma unroll
-          for (int u = 0; u < kDisGroup; ++u) {
-            const int v = v0 + u * kCompute;
-            if (v >= c.vecs) continue;
-            if (kMode == kDistillGrad) vector(v, q[u]);
-            else q[u] = stage[v];
+            for (int u = 0; u < kDisGroup; ++u)
+              if (v0 + u * kCompute < c.vecs) q[u] = stage[v0 + u * kCompute];
           }
 #pragma unroll
           for (int u = 0; u < kDisGroup; ++u) {
@@ -529,8 +556,9 @@ cudaError_t resident_teams(const cudaLaunchConfig_t &cfg, int dev, int team, int
   return cudaSuccess;
 }
 
-size_t distill_smem(int slice, int top, size_t bytes) {
-  return size_t(slice) * bytes + 16 + 2 * size_t((top + 3) & ~3) * 16 + 2 * (size_t(slice) / 32 + 2) * 4;
+template <int kCompute> size_t distill_smem(int slice, const ds41_b200_distill_args &a, size_t bytes) {
+  return size_t(slice) * bytes + 16 + 2 * size_t((a.top + 3) & ~3) * 16 + 2 * size_t(distill_bit_words<kCompute>(slice * int(bytes))) * 4 +
+         (a.mask ? size_t(slice) / 32 * 4 : 0);
 }
 
 template <class T, int kMode, int kCompute>
@@ -541,7 +569,7 @@ cudaError_t launch_distill(const DistillParams &p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(p.team));
   cfg.blockDim = dim3(kCompute + 64);
-  cfg.dynamicSmemBytes = distill_smem(p.slice, p.a.top, sizeof(T));
+  cfg.dynamicSmemBytes = distill_smem<kCompute>(p.slice, p.a, sizeof(T));
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -560,12 +588,12 @@ cudaError_t launch_distill(const DistillParams &p, cudaStream_t stream) {
 template <class T, int kMode>
 cudaError_t launch_distill(DistillParams &d, cudaStream_t stream) {
   constexpr int kSmall = 64 * kDisVectors * 16 / int(sizeof(T)), kLarge = 4 * kSmall;   // ids of a CTA
-  const int vocab = d.a.vocab, top = d.a.top;
+  const int vocab = d.a.vocab;
   // CTAs per row: as few as hold it, three CTAs to an SM where eight of them can, and for batches that leave SMs idle up to eight, of at least
   // 4096 ids each
   auto slice = [&](int team) { return ((vocab + team - 1) / team + 31) & ~31; };
   d.team = 1;
-  while (d.team < 8 && (slice(d.team) > kLarge || distill_smem(slice(d.team), top, sizeof(T)) > 74 * 1024)) ++d.team;
+  while (d.team < 8 && (slice(d.team) > kLarge || distill_smem<256>(slice(d.team), d.a, sizeof(T)) > 74 * 1024)) ++d.team;
   while (d.team < 8 && 2LL * d.a.rows * d.team <= 148 && vocab > d.team * 4096) ++d.team;
   d.slice = slice(d.team);
   return d.slice <= kSmall ? launch_distill<T, kMode, 64>(d, stream) : launch_distill<T, kMode, 256>(d, stream);
