@@ -12,7 +12,6 @@
 // asynchronous copy on (no barrier between copy and use), and where it has written a vector's gradient it starts the copy of the
 // next row's.  Two more warps are a row ahead: one gathers and reduces the next row's list, the other sets the bits of the ids
 // that count into the sum and, a row behind, takes the loss in FP64.  Three CTAs share an SM, each at another point of its row.
-#include "packed_fma.cuh"
 #include "row_types.cuh"
 #include "row_team.cuh"
 #include "host_error.h"
@@ -62,6 +61,13 @@ __device__ __forceinline__ float exp2_approx(float x) {   // 2 ulp; 0 for -inf a
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// An exponent of two below which, and above whose negative, a product of logit and log2(e) / T is taken as it is: the power of
+// x c - r with r = m c rounded is one fused multiply-add, its argument as exact as that of (x - m) c, if the rounding of r is made good for
+// once a row.  Beyond (rows of a type's lowest values) it is (x - m) c.
+constexpr float kDisNear = 1e37f;
+__device__ __forceinline__ bool near_exponent(float r) { return fabsf(r) < kDisNear; }
+__device__ __forceinline__ float excess(float m, float c, float r) { return near_exponent(r) ? fmaf(m, c, -r) : 0.f; }
 
 // Out of line, once each: what runs a few times a row shall not push the loops out of the instruction cache.
 __device__ __noinline__ double exp_of(double x) { return exp(x); }
@@ -368,7 +374,7 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
       const DistillSlice<T> c(p, row, begin, len), c_next(p, has_next ? next : row, begin, len);
       const bool skip = skipped(r), ahead = has_next && !skipped(s.rows[(turn + 1) & 3]);
       const uint32_t *const in_sum = bits + (turn & 1) * bits_room + tid;
-      const float2x c2 = pack_f32x2(p.log2e_t, p.log2e_t);
+      const float log2e_t = p.log2e_t;
       T *const grad = kMode == kDistillLoss ? nullptr : static_cast<T *>(a.grad) + size_t(row) * size_t(a.grad_stride) + begin;
       const bool by_vectors = kMode != kDistillLoss && int((reinterpret_cast<uintptr_t>(grad) / sizeof(T)) % kVec) == c.lead;
       auto put = [&](int v, const uint4 &q) {
@@ -411,39 +417,44 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
       };
 
       // ---- maximum and sum of the ids outside the list
-      float high = -FLT_MAX;
-      float2x sums[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
+      float high = -FLT_MAX, high_c = -INFINITY, sums[4] = {0.f, 0.f, 0.f, 0.f};   // (relative to high_c)
       auto add = [&](int v0) {
         uint4 q[kDisGroup];
         take(v0, std::integral_constant<bool, kMode == kDistillBoth>{}, q);
         const float top = R::largest(q);
         if (top > high) {
-          const float down = exp2_approx((high - top) * p.log2e_t);
-          sums[0] = mul_f32x2(sums[0], pack_f32x2(down, down));
-          sums[1] = mul_f32x2(sums[1], pack_f32x2(down, down));
-          high = top;
+          const float top_c = top * log2e_t;
+          const float down = exp2_approx(near_exponent(top_c) && near_exponent(high_c) ? high_c - top_c : (high - top) * log2e_t);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sums[i] *= down;
+          high = top; high_c = top_c;
         }
-        const float2x minus = pack_f32x2(-high, -high);
+        if (near_exponent(high_c)) {
 #pragma unroll
-        for (int u = 0; u < kDisGroup; ++u) {
-          float y[kVec];
-          R::unpack(q[u], y);
+          for (int u = 0; u < kDisGroup; ++u) {
+            float y[kVec];
+            R::unpack(q[u], y);
 #pragma unroll
-          for (int k = 0; k < kVec; k += 2) {
-            float e0, e1;
-            unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(y[k], y[k + 1]), minus), c2), e0, e1);
-            sums[k / 2 % 2] = add_f32x2(sums[k / 2 % 2], pack_f32x2(exp2_approx(e0), exp2_approx(e1)));
+            for (int k = 0; k < kVec; ++k) sums[k % 4] += exp2_approx(fmaf(y[k], log2e_t, -high_c));
+          }
+        } else {
+#pragma unroll 1
+          for (int u = 0; u < kDisGroup; ++u) {
+            float y[kVec];
+            R::unpack(u == 0 ? q[0] : u == 1 ? q[1] : u == 2 ? q[2] : q[3], y);
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) sums[k % 4] += exp2_approx((y[k] - high) * log2e_t);
           }
         }
       };
       if (kMode == kDistillLoss) run(Yes{}, Yes{}, add);
       if (kMode == kDistillBoth && !skip) run(Yes{}, No{}, add);
       if (kMode != kDistillGrad) {
-        float s0, s1, all = high;
-        unpack_f32x2(add_f32x2(sums[0], sums[1]), s0, s1);
+        float all = high;
 #pragma unroll
         for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
-        float sum = (s0 + s1) * exp2_approx((high - all) * p.log2e_t);
+        float sum = ((sums[0] + sums[1]) + (sums[2] + sums[3])) * exp2_approx(-excess(high, log2e_t, high_c));   // relative to high
+        sum *= exp2_approx((high - all) * log2e_t);
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) s.sums[turn & 1][warp] = make_float2(all, sum);
@@ -455,7 +466,7 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
         for (int w = lane; w < kWarps * p.team; w += 32) {            // (64 at most: two a lane, of the same order everywhere)
           const float2 its = team_read(&s.sums[turn & 1][w % kWarps], w / kWarps);
           const float most = fmaxf(rest_max, its.x);
-          rest_sum = rest_sum * exp2_approx((rest_max - most) * p.log2e_t) + its.y * exp2_approx((its.x - most) * p.log2e_t);
+          rest_sum = rest_sum * exp2_approx((rest_max - most) * log2e_t) + its.y * exp2_approx((its.x - most) * p.log2e_t);
           rest_max = most;
         }
         float all = rest_max;
@@ -496,7 +507,13 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
         uint32_t filling = 0u;
         if (!skip && reject != DS41_B200_ROW_EMPTY)
           filling = sizeof(T) == 4 ? *reinterpret_cast<const uint32_t *>(&nan) : *reinterpret_cast<const uint16_t *>(&nan) * 0x10001u;
-        const float2x minus = pack_f32x2(-rest_max, -rest_max), coef2 = pack_f32x2(coef, coef);
+        // 16-bit types: the factor's size goes into the exponent, its sign into the words (exponents below 256 are off by 2^-17, a power
+        // by 2^-17, which is little beside the rounding to 16 bits)
+        const float rest_c = rest_max * log2e_t;
+        const bool close = sizeof(T) == 4 ? near_exponent(rest_c) : fabsf(rest_c) < 256.f;
+        const float shift = sizeof(T) == 4 ? 0.f : log2f(fabsf(coef)), size = sizeof(T) == 4 ? coef * exp2_approx(-excess(rest_max, log2e_t, rest_c)) : 1.f;
+        const float offset = sizeof(T) == 4 ? -rest_c : shift - rest_c - excess(rest_max, log2e_t, rest_c);
+        const uint32_t sign = sizeof(T) != 4 && coef < 0.f ? 0x80008000u : 0u;
         auto step = [&](int v0) {
           uint4 q[kDisGroup];
           if (kMode == kDistillGrad) {
@@ -512,13 +529,20 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
             if (v >= c.vecs) break;
             float y[kVec];
             R::unpack(q[u], y);
+            if (close) {
 #pragma unroll
-            for (int k = 0; k < kVec; k += 2) {
-              float e0, e1;
-              unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(y[k], y[k + 1]), minus), c2), e0, e1);
-              unpack_f32x2(mul_f32x2(pack_f32x2(exp2_approx(e0), exp2_approx(e1)), coef2), y[k], y[k + 1]);
+              for (int k = 0; k < kVec; ++k) y[k] = exp2_approx(fmaf(y[k], log2e_t, offset));
+            } else {
+#pragma unroll
+              for (int k = 0; k < kVec; ++k) y[k] = exp2_approx((y[k] - rest_max) * log2e_t + shift);
             }
-            put(v, fill ? make_uint4(filling, filling, filling, filling) : R::pack(y));
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+              for (int k = 0; k < kVec; ++k) y[k] *= size;
+            }
+            uint4 g = R::pack(y);
+            if constexpr (sizeof(T) != 4) g = make_uint4(g.x ^ sign, g.y ^ sign, g.z ^ sign, g.w ^ sign);
+            put(v, fill ? make_uint4(filling, filling, filling, filling) : g);
           }
         };
         run(std::integral_constant<bool, kMode == kDistillGrad>{}, Yes{}, step);

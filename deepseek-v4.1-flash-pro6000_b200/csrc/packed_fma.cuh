@@ -21,16 +21,6 @@ __device__ __forceinline__ float2x fma_f32x2(float2x a, float2x b, float2x c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
-__device__ __forceinline__ float2x add_f32x2(float2x a, float2x b) {
-  float2x d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ float2x mul_f32x2(float2x a, float2x b) {
-  float2x d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 // The two BF16 values of a 32-bit word, promoted to FP32.
 __device__ __forceinline__ float2x promote_bf16x2(uint32_t w) {
   return pack_f32x2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
