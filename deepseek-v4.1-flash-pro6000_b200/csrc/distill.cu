@@ -38,9 +38,6 @@ struct DistillParams {
   float log2e_t;                              // log2(e) / T
 };
 
-__device__ __forceinline__ void copy16_async(const void *to, const void *from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from) : "memory");
-}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void copies_wait(int left) {
   switch (left) {
@@ -90,20 +87,26 @@ struct DistillSmem {
   float2 result[2];                           // (maximum, sum) of the row's ids outside the list
 };
 
-// A row's slice as this CTA sees it.  Place 0 is where the vector of its first id begins.
-template <class T>
+// A row's slice as one of its CTA's threads sees it, which takes vectors t, t + kCompute, ... of it ("at" 0, kCompute, ...).  Place 0 is
+// where the vector of the slice's first id begins.
+template <class T, int kCompute>
 struct DistillSlice {
+  static constexpr int kVec = RowType<T>::kVec;
   const T *x;
-  int lead, vecs, first_whole, wholes;        // vectors; those of which no id is another slice's
-  __device__ __forceinline__ DistillSlice(const DistillParams &p, int row, int begin, int len) {
-    constexpr int kVec = RowType<T>::kVec;
+  const uint4 *from;                          // the thread's first vector
+  int lead, vecs;                             // vectors of the slice
+  int mine, wholes;                           // its vectors are the slice's below `mine`, and hold no other slice's ids below `wholes`
+  bool cut;                                   // ... but for the first one
+  __device__ __forceinline__ DistillSlice(const DistillParams &p, int row, int begin, int len, int t) {
     x = static_cast<const T *>(p.a.logits) + size_t(row) * size_t(p.a.logits_stride) + begin;
     lead = int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % kVec);
     vecs = (lead + len + kVec - 1) / kVec;
-    first_whole = lead ? 1 : 0;
-    wholes = max(0, (lead + len) / kVec - first_whole);
+    from = reinterpret_cast<const uint4 *>(x - lead) + t;
+    mine = vecs - t; wholes = (lead + len) / kVec - t;
+    cut = lead && t == 0;
   }
-  __device__ __forceinline__ bool whole(int v) const { return unsigned(v - first_whole) < unsigned(wholes); }
+  __device__ __forceinline__ bool whole(int at) const { return at < wholes && !(cut && at == 0); }
+  __device__ __forceinline__ bool any_partial() const { return cut || wholes < mine; }
 };
 
 // A vector that is not whole comes and goes by its ids, `from` .. `to`.
@@ -145,13 +148,20 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
 
   auto row_scale = [&](int row) { return kMode != kDistillLoss && a.row_scale && row < a.rows ? load_input(a.row_scale + row) : 1.f; };
   auto skipped = [&](const DistillRow &r) { return kMode != kDistillLoss && r.scale == 0.f; };
-  // the copies of a group of the thread's vectors, from v0 on
-  auto start_copies = [&](const DistillSlice<T> &c, int v0) {
+  // the copies of a group of the thread's vectors
+  auto start_copies = [&](const DistillSlice<T, kCompute> &c, int at) {
+    const uint32_t to = uint32_t(__cvta_generic_to_shared(stage + tid + at));
 #pragma unroll
-    for (int u = 0; u < kDisGroup; ++u) {
-      const int v = v0 + u * kCompute;
-      if (c.whole(v)) copy16_async(&stage[v], reinterpret_cast<const uint4 *>(c.x - c.lead) + v);
-      else if (v < c.vecs) copy_ids<T>(reinterpret_cast<T *>(stage) + c.lead, c.x, max(0, v * kVec - c.lead), min(len, (v + 1) * kVec - c.lead));
+    for (int u = 0; u < kDisGroup; ++u)
+      if (c.whole(at + u * kCompute))
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + u * kCompute * 16), "l"(c.from + at + u * kCompute) : "memory");
+    if (c.any_partial()) {
+#pragma unroll 1
+      for (int i = at; i < min(c.mine, at + kDisGroup * kCompute); i += kCompute)
+        if (!c.whole(i)) {
+          const int v = tid + i;
+          copy_ids<T>(reinterpret_cast<T *>(stage) + c.lead, c.x, max(0, v * kVec - c.lead), min(len, (v + 1) * kVec - c.lead));
+        }
     }
     copies_commit();
   };
@@ -268,7 +278,7 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
       if (kMode == kDistillGrad) r.stats = reinterpret_cast<const float4 *>(a.stats)[row];
     }
     barrier_of<2, 64>();                      // (the bits are set)
-    const DistillSlice<T> c(p, row, begin, len);
+    const DistillSlice<T, kCompute> c(p, row, begin, len, 0);
     uint32_t *const out = bits + (turn & 1) * bits_room;
 #pragma unroll 1
     for (int k = 0; k < own; ++k) {
@@ -282,7 +292,7 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
   };
   // ---- by the other: the bits of its allowed ids
   auto take_bits = [&](int row, int turn) {
-    const DistillSlice<T> c(p, row, begin, len);
+    const DistillSlice<T, kCompute> c(p, row, begin, len, 0);
     uint32_t *const out = bits + (turn & 1) * bits_room;
     if (a.mask) {
       const uint32_t *from = a.mask + size_t(row) * size_t(a.mask_stride) + begin / 32;
@@ -365,62 +375,56 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
       if (together && has) team_wait();
     } else if (!has) {
       if (has_next && row_scale(next) != 0.f) {
-        const DistillSlice<T> c(p, next, begin, len);
+        const DistillSlice<T, kCompute> c(p, next, begin, len, tid);
 #pragma unroll 1
-        for (int g = 0; g < kDisGroups; ++g) start_copies(c, tid + g * kDisGroup * kCompute);
+        for (int g = 0; g < kDisGroups; ++g) start_copies(c, g * kDisGroup * kCompute);
       }
     } else {
       const DistillRow &r = s.rows[turn & 3];
-      const DistillSlice<T> c(p, row, begin, len), c_next(p, has_next ? next : row, begin, len);
+      const DistillSlice<T, kCompute> c(p, row, begin, len, tid), c_next(p, has_next ? next : row, begin, len, tid);
       const bool skip = skipped(r), ahead = has_next && !skipped(s.rows[(turn + 1) & 3]);
       const uint32_t *const in_sum = bits + (turn & 1) * bits_room + tid;
       const float log2e_t = p.log2e_t;
       T *const grad = kMode == kDistillLoss ? nullptr : static_cast<T *>(a.grad) + size_t(row) * size_t(a.grad_stride) + begin;
       const bool by_vectors = kMode != kDistillLoss && int((reinterpret_cast<uintptr_t>(grad) / sizeof(T)) % kVec) == c.lead;
-      auto put = [&](int v, const uint4 &q) {
-        if (by_vectors && c.whole(v)) {
-          reinterpret_cast<uint4 *>(grad - c.lead)[v] = q;
-        } else {                              // (by way of the stage, where the vector is not needed any more)
-          stage[v] = q;
-          copy_ids<T>(grad, reinterpret_cast<const T *>(stage) + c.lead, max(0, v * kVec - c.lead), min(len, (v + 1) * kVec - c.lead));
-        }
-      };
-      // f(first vector) over the thread's vectors by groups.  arrive: as their copies do; start_next: behind each
-      // group the copies of the next row's, so that as many groups are on their way as before
+      // f(at) over the thread's vectors by groups.  arrive: as their copies do; start_next: behind each group the copies of the next
+      // row's, so that as many groups are on their way as before
       auto run = [&](auto arrive, auto start_next, auto f) {
 #pragma unroll 1
         for (int g = 0; g < kDisGroups; ++g) {
-          const int v0 = tid + g * kDisGroup * kCompute;
+          const int at = g * kDisGroup * kCompute;
           if (arrive.value) copies_wait(kDisGroups - 1 - (start_next.value && ahead ? 0 : g));
-          if (v0 < c.vecs) f(v0);
-          if (start_next.value && ahead) start_copies(c_next, v0);
+          if (at < c.mine) f(at);
+          if (start_next.value && ahead) start_copies(c_next, at);
         }
       };
       using Yes = std::true_type;
       using No = std::false_type;
       // a group of vectors; ids that are not in the sum are -inf.  kKeep: in the stage too
-      auto take = [&](int v0, auto keep, uint4 (&q)[kDisGroup]) {
-        uint32_t in = in_sum[(v0 - tid) / kDisGroup];
+      auto take = [&](int at, auto keep, uint4 (&q)[kDisGroup]) {
+        uint32_t in = in_sum[at / kDisGroup];
+        uint4 *const here = stage + tid + at;
 #pragma unroll
         for (int u = 0; u < kDisGroup; ++u) {
           q[u] = R::nothing();
-          if (v0 + u * kCompute < c.vecs) q[u] = stage[v0 + u * kCompute];
+          if (at + u * kCompute < c.mine) q[u] = here[u * kCompute];
         }
         if (sizeof(T) == 4) in |= 0xffff0000u;
         if (in != ~0u) {
 #pragma unroll
           for (int u = 0; u < kDisGroup; ++u) {
+            if (((in >> (u * kVec)) & kAll) == kAll) continue;
             q[u] = R::only(q[u], in >> (u * kVec));
-            if (keep.value && v0 + u * kCompute < c.vecs) stage[v0 + u * kCompute] = q[u];
+            if (keep.value && at + u * kCompute < c.mine) here[u * kCompute] = q[u];
           }
         }
       };
 
       // ---- maximum and sum of the ids outside the list
       float high = -FLT_MAX, high_c = -INFINITY, sums[4] = {0.f, 0.f, 0.f, 0.f};   // (relative to high_c)
-      auto add = [&](int v0) {
+      auto add = [&](int at) {
         uint4 q[kDisGroup];
-        take(v0, std::integral_constant<bool, kMode == kDistillBoth>{}, q);
+        take(at, std::integral_constant<bool, kMode == kDistillBoth>{}, q);
         const float top = R::largest(q);
         if (top > high) {
           const float top_c = top * log2e_t;
@@ -503,10 +507,6 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
         const double factor = double(r.scale) * t;
         const float tail = any ? float(r.rest * inverse) : 0.f, coef = any ? float(factor) * (q_rest - tail) / rest_sum : 0.f;
         const bool fill = skip || reject != 0;
-        const T nan = R::store(__int_as_float(0x7fffffff));
-        uint32_t filling = 0u;
-        if (!skip && reject != DS41_B200_ROW_EMPTY)
-          filling = sizeof(T) == 4 ? *reinterpret_cast<const uint32_t *>(&nan) : *reinterpret_cast<const uint16_t *>(&nan) * 0x10001u;
         // 16-bit types: the factor's size goes into the exponent, its sign into the words (exponents below 256 are off by 2^-17, a power
         // by 2^-17, which is little beside the rounding to 16 bits)
         const float rest_c = rest_max * log2e_t;
@@ -514,19 +514,18 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
         const float shift = sizeof(T) == 4 ? 0.f : log2f(fabsf(coef)), size = sizeof(T) == 4 ? coef * exp2_approx(-excess(rest_max, log2e_t, rest_c)) : 1.f;
         const float offset = sizeof(T) == 4 ? -rest_c : shift - rest_c - excess(rest_max, log2e_t, rest_c);
         const uint32_t sign = sizeof(T) != 4 && coef < 0.f ? 0x80008000u : 0u;
-        auto step = [&](int v0) {
+        uint4 *const to = reinterpret_cast<uint4 *>(grad - c.lead) + tid;
+        auto step = [&](int at) {
           uint4 q[kDisGroup];
           if (kMode == kDistillGrad) {
-            take(v0, No{}, q);
+            take(at, No{}, q);
           } else {
 #pragma unroll
             for (int u = 0; u < kDisGroup; ++u)
-              if (v0 + u * kCompute < c.vecs) q[u] = stage[v0 + u * kCompute];
+              if (at + u * kCompute < c.mine) q[u] = stage[tid + at + u * kCompute];
           }
 #pragma unroll
           for (int u = 0; u < kDisGroup; ++u) {
-            const int v = v0 + u * kCompute;
-            if (v >= c.vecs) break;
             float y[kVec];
             R::unpack(q[u], y);
             if (close) {
@@ -540,12 +539,37 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
 #pragma unroll
               for (int k = 0; k < kVec; ++k) y[k] *= size;
             }
-            uint4 g = R::pack(y);
-            if constexpr (sizeof(T) != 4) g = make_uint4(g.x ^ sign, g.y ^ sign, g.z ^ sign, g.w ^ sign);
-            put(v, fill ? make_uint4(filling, filling, filling, filling) : g);
+            q[u] = R::pack(y);
+            if constexpr (sizeof(T) != 4) q[u] = make_uint4(q[u].x ^ sign, q[u].y ^ sign, q[u].z ^ sign, q[u].w ^ sign);
+            if (by_vectors && c.whole(at + u * kCompute)) to[at + u * kCompute] = q[u];
+          }
+          if (!by_vectors || c.any_partial()) {             // by way of the stage, where the vector is not needed any more
+#pragma unroll
+            for (int u = 0; u < kDisGroup; ++u) {
+              const int i = at + u * kCompute, v = tid + i;
+              if (i >= c.mine || (by_vectors && c.whole(i))) continue;
+              stage[v] = q[u];
+              copy_ids<T>(grad, reinterpret_cast<const T *>(stage) + c.lead, max(0, v * kVec - c.lead), min(len, (v + 1) * kVec - c.lead));
+            }
           }
         };
-        run(std::integral_constant<bool, kMode == kDistillGrad>{}, Yes{}, step);
+        if (!fill) {
+          run(std::integral_constant<bool, kMode == kDistillGrad>{}, Yes{}, step);
+        } else {                              // (a row that was rejected, or is padding)
+          if (!skip) copies_wait(0);
+          run(No{}, Yes{}, [](int) {});
+          const T each = !skip && reject != DS41_B200_ROW_EMPTY ? R::store(__int_as_float(0x7fffffff)) : R::store(0.f);
+          const T pair[2] = {each, each};
+          const uint32_t w = sizeof(T) == 4 ? *reinterpret_cast<const uint32_t *>(&each) : *reinterpret_cast<const uint32_t *>(pair);
+#pragma unroll 1
+          for (int i = 0; i < c.mine; i += kCompute) {
+            if (by_vectors && c.whole(i)) to[i] = make_uint4(w, w, w, w);
+            else {
+#pragma unroll 1
+              for (int k = max(0, (tid + i) * kVec - c.lead); k < min(len, (tid + i + 1) * kVec - c.lead); ++k) grad[k] = each;
+            }
+          }
+        }
         if (!fill) {
           barrier_of<1, kCompute>();          // (zeros stand where listed ids are)
           for (int e = tid; e < a.top; e += kCompute) {
