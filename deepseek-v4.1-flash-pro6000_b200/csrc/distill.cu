@@ -83,8 +83,9 @@ struct DistillRow {
 template <int kCompute>
 struct DistillSmem {
   DistillRow rows[4];                         // by the number of the row's turn: the last one, this one, the next two
-  float2 sums[2][kCompute / 32];              // every warp's (maximum, sum), read by the whole team
+  float2 sums[4][kCompute / 32];              // every warp's (maximum, sum), read by the team
   float2 result[2];                           // (maximum, sum) of the row's ids outside the list
+  float2 all[2];                              // of all its ids: the maximum, 1 / the sum; a NaN where the gradient has no listed ids to set
 };
 
 // A row's slice as one of its CTA's threads sees it, which takes vectors t, t + kCompute, ... of it ("at" 0, kCompute, ...).  Place 0 is
@@ -357,14 +358,59 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
     if (a.stats) reinterpret_cast<float4 *>(a.stats)[row] = stats;
   };
 
-  const bool together = p.team > 1 && (kMode != kDistillGrad || p.in_place);   // the team's CTAs wait for one another every turn
+  // (maximum, sum) of the ids outside the list of the turn's row, from the whole team's warps: 64 at most, in the same order everywhere
+  auto combine = [&](int turn) {
+    float most = -FLT_MAX, sum = 0.f;
+    for (int w = lane; w < kWarps * p.team; w += 32) {
+      const float2 its = team_read(&s.sums[turn & 3][w % kWarps], w / kWarps);
+      const float high = fmaxf(most, its.x);
+      sum = sum * exp2_approx((most - high) * p.log2e_t) + its.y * exp2_approx((its.x - high) * p.log2e_t);
+      most = high;
+    }
+    float all = most;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
+    sum *= exp2_approx((most - all) * p.log2e_t);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return make_float2(all, sum);
+  };
+  // ---- the gradient of the listed ids of a row whose other ids are written
+  auto set_listed = [&](int row, int turn) {
+    const DistillRow &r = s.rows[turn & 3];
+    const float2 all = s.all[turn & 1];
+    if (!(all.y == all.y)) return;
+    const double inverse = s.result[turn & 1].y != 0.f ? r.inverse_rest : r.inverse, factor = double(r.scale) * t;
+    T *const grad = static_cast<T *>(a.grad) + size_t(row) * size_t(a.grad_stride) + begin;
+#pragma unroll 1
+    for (int e = lane; e < a.top; e += 32) {
+      const unsigned local = unsigned(ids[(turn & 1) * top_room + e]) - unsigned(begin);
+      if (local >= unsigned(len)) continue;
+      const float q = exp2_approx((zs[(turn & 1) * top_room + e] - all.x) * p.log2e_t) * all.y;
+      grad[local] = R::store(float(factor * (double(q) - weights[(turn & 1) * top_room + e] * inverse)));
+    }
+    __syncwarp();                             // (the list's memory is the next but one row's)
+  };
+
+  // The team's CTAs wait for one another once a row: for each other's sums, and until each has read of the row what it needs of other
+  // slices.  The loss alone is not waited for by the compute warps until they have the next row's sums.
+  const bool together = p.team > 1 && (kMode != kDistillGrad || p.in_place);
   const int turns = (a.rows - own_team + teams - 1) / teams;
   for (int turn = -1; turn <= turns; ++turn) {  // (one ahead for the first list and copies, one behind for the last loss)
     const int row = own_team + turn * teams, next = row + teams;
     const bool has = turn >= 0 && turn < turns, has_next = turn + 1 < turns;
-    if (warp >= kWarps) {                     // a row ahead
+    if (warp >= kWarps) {                     // a row ahead, and a row behind
+      if (kMode == kDistillLoss) {
+        if (together && turn > 0) team_wait();
+        if (warp > kWarps && turn > 0 && rank == 0) {
+          const float2 both = combine(turn - 1);
+          if (lane == 0) s.result[(turn - 1) & 1] = both;
+          __syncwarp();
+        }
+      }
       if (together && has) team_arrive();
       if (warp == kWarps) {
+        if (kMode != kDistillLoss && turn > 0) set_listed(row - teams, turn - 1);
         if (has_next) take_list(next, turn + 1);
       } else {
         if (lane == 0) s.rows[(turn + 2) & 3].scale = row_scale(next + teams);
@@ -372,8 +418,9 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
         if (has_next) take_bits(next, turn + 1);
         if (kMode != kDistillGrad && rank == 0 && lane == 0 && turn > 0) finish(row - teams, turn - 1);
       }
-      if (together && has) team_wait();
+      if (kMode != kDistillLoss && together && has) team_wait();
     } else if (!has) {
+      if (kMode == kDistillLoss && together && turn > 0) team_wait();
       if (has_next && row_scale(next) != 0.f) {
         const DistillSlice<T, kCompute> c(p, next, begin, len, tid);
 #pragma unroll 1
@@ -400,32 +447,20 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
       };
       using Yes = std::true_type;
       using No = std::false_type;
-      // a group of vectors; ids that are not in the sum are -inf.  kKeep: in the stage too
-      auto take = [&](int at, auto keep, uint4 (&q)[kDisGroup]) {
-        uint32_t in = in_sum[at / kDisGroup];
-        uint4 *const here = stage + tid + at;
-#pragma unroll
-        for (int u = 0; u < kDisGroup; ++u) {
-          q[u] = R::nothing();
-          if (at + u * kCompute < c.mine) q[u] = here[u * kCompute];
-        }
-        if (sizeof(T) == 4) in |= 0xffff0000u;
-        if (in != ~0u) {
-#pragma unroll
-          for (int u = 0; u < kDisGroup; ++u) {
-            if (((in >> (u * kVec)) & kAll) == kAll) continue;
-            q[u] = R::only(q[u], in >> (u * kVec));
-            if (keep.value && at + u * kCompute < c.mine) here[u * kCompute] = q[u];
-          }
-        }
+      // one vector of a group whose bits are `in`, ids that are not in the sum as -inf; keep: in the stage too
+      auto take = [&](int at, int u, uint32_t in, bool keep) {
+        uint4 *const here = stage + tid + at + u * kCompute;
+        const unsigned some = (in >> (u * kVec)) & kAll;
+        if (some == kAll) return *here;
+        const uint4 q = R::only(*here, some);
+        if (keep) *here = q;
+        return q;
       };
+      constexpr uint32_t kNone = sizeof(T) == 4 ? 0xffff0000u : 0u;     // (a word's bits that are no vector's)
 
       // ---- maximum and sum of the ids outside the list
       float high = -FLT_MAX, high_c = -INFINITY, sums[4] = {0.f, 0.f, 0.f, 0.f};   // (relative to high_c)
-      auto add = [&](int at) {
-        uint4 q[kDisGroup];
-        take(at, std::integral_constant<bool, kMode == kDistillBoth>{}, q);
-        const float top = R::largest(q);
+      auto raise = [&](float top) {
         if (top > high) {
           const float top_c = top * log2e_t;
           const float down = exp2_approx(near_exponent(top_c) && near_exponent(high_c) ? high_c - top_c : (high - top) * log2e_t);
@@ -433,21 +468,37 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
           for (int i = 0; i < 4; ++i) sums[i] *= down;
           high = top; high_c = top_c;
         }
-        if (near_exponent(high_c)) {
+      };
+      auto add = [&](int at) {
+        const uint32_t in = in_sum[at / kDisGroup] | kNone;
+        bool fast = in == ~0u && at + (kDisGroup - 1) * kCompute < c.mine;
+        if (fast) {
+          uint4 q[kDisGroup];
 #pragma unroll
-          for (int u = 0; u < kDisGroup; ++u) {
-            float y[kVec];
-            R::unpack(q[u], y);
+          for (int u = 0; u < kDisGroup; ++u) q[u] = stage[tid + at + u * kCompute];
+          raise(R::largest(q));
+          fast = near_exponent(high_c);
+          if (fast) {
 #pragma unroll
-            for (int k = 0; k < kVec; ++k) sums[k % 4] += exp2_approx(fmaf(y[k], log2e_t, -high_c));
+            for (int u = 0; u < kDisGroup; ++u) {
+              float y[kVec];
+              R::unpack(q[u], y);
+#pragma unroll
+              for (int k = 0; k < kVec; ++k) sums[k % 4] += exp2_approx(fmaf(y[k], log2e_t, -high_c));
+            }
           }
-        } else {
+        }
+        if (!fast) {                          // some ids of the group are out, or not there, or far from the others
 #pragma unroll 1
-          for (int u = 0; u < kDisGroup; ++u) {
+          for (int u = 0; u < kDisGroup && at + u * kCompute < c.mine; ++u) {
+            const uint4 q[1] = {take(at, u, in, kMode == kDistillBoth)};
+            raise(R::largest(q));
             float y[kVec];
-            R::unpack(u == 0 ? q[0] : u == 1 ? q[1] : u == 2 ? q[2] : q[3], y);
+            R::unpack(q[0], y);
+            const float factor = near_exponent(high_c) ? 1.f : log2e_t, scaled = near_exponent(high_c) ? log2e_t : 1.f;
+            const float minus = near_exponent(high_c) ? -high_c : -high;
 #pragma unroll
-            for (int k = 0; k < kVec; ++k) sums[k % 4] += exp2_approx((y[k] - high) * log2e_t);
+            for (int k = 0; k < kVec; ++k) sums[k % 4] += exp2_approx(fmaf(y[k], scaled, minus) * factor);
           }
         }
       };
@@ -461,26 +512,22 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
         sum *= exp2_approx((high - all) * log2e_t);
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) s.sums[turn & 1][warp] = make_float2(all, sum);
+        if (lane == 0) s.sums[turn & 3][warp] = make_float2(all, sum);
       }
-      if (together) team_barrier();           // every CTA has its sums, and has read of the row what it needs of other slices
-      else if (kMode != kDistillGrad) barrier_of<1, kCompute>();
       float rest_max = -FLT_MAX, rest_sum = 0.f;
-      if (kMode != kDistillGrad) {
-        for (int w = lane; w < kWarps * p.team; w += 32) {            // (64 at most: two a lane, of the same order everywhere)
-          const float2 its = team_read(&s.sums[turn & 1][w % kWarps], w / kWarps);
-          const float most = fmaxf(rest_max, its.x);
-          rest_sum = rest_sum * exp2_approx((rest_max - most) * log2e_t) + its.y * exp2_approx((its.x - most) * p.log2e_t);
-          rest_max = most;
+      if (kMode == kDistillLoss) {
+        if (together) {
+          if (turn > 0) team_wait();          // (for the row before)
+          team_arrive();
         }
-        float all = rest_max;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
-        rest_sum *= exp2_approx((rest_max - all) * p.log2e_t);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) rest_sum += __shfl_xor_sync(0xffffffffu, rest_sum, o);
-        rest_max = all;
-        if (tid == 0) s.result[turn & 1] = make_float2(rest_max, rest_sum);
+      } else if (together) {
+        team_barrier();
+      } else if (kMode == kDistillBoth) {
+        barrier_of<1, kCompute>();
+      }
+      if (kMode == kDistillBoth) {
+        const float2 both = combine(turn);
+        rest_max = both.x; rest_sum = both.y;
       }
 
       // ---- the gradient
@@ -503,10 +550,12 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
           q_rest = part * inverse_sum;
           if (!reject && !(rest_sum < INFINITY)) reject = DS41_B200_ROW_NONFINITE;
         }
-        const double inverse = any ? r.inverse_rest : r.inverse;
-        const double factor = double(r.scale) * t;
-        const float tail = any ? float(r.rest * inverse) : 0.f, coef = any ? float(factor) * (q_rest - tail) / rest_sum : 0.f;
+        const float tail = any ? float(r.rest * r.inverse_rest) : 0.f, coef = any ? r.scale * float(t) * (q_rest - tail) / rest_sum : 0.f;
         const bool fill = skip || reject != 0;
+        if (tid == 0) {
+          s.result[turn & 1] = make_float2(rest_max, rest_sum);
+          s.all[turn & 1] = make_float2(largest, fill ? __int_as_float(0x7fffffff) : inverse_sum);
+        }
         // 16-bit types: the factor's size goes into the exponent, its sign into the words (exponents below 256 are off by 2^-17, a power
         // by 2^-17, which is little beside the rounding to 16 bits)
         const float rest_c = rest_max * log2e_t;
@@ -515,41 +564,46 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
         const float offset = sizeof(T) == 4 ? -rest_c : shift - rest_c - excess(rest_max, log2e_t, rest_c);
         const uint32_t sign = sizeof(T) != 4 && coef < 0.f ? 0x80008000u : 0u;
         uint4 *const to = reinterpret_cast<uint4 *>(grad - c.lead) + tid;
+        const float rest_scaled = close ? log2e_t : 1.f, rest_factor = close ? 1.f : log2e_t;
+        const float rest_offset = close ? offset : -rest_max, rest_shift = close ? 0.f : shift;
+        auto finish_vector = [&](float (&y)[kVec]) {
+          if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) y[k] *= size;
+          }
+          uint4 g = R::pack(y);
+          if constexpr (sizeof(T) != 4) g = make_uint4(g.x ^ sign, g.y ^ sign, g.z ^ sign, g.w ^ sign);
+          return g;
+        };
         auto step = [&](int at) {
-          uint4 q[kDisGroup];
-          if (kMode == kDistillGrad) {
-            take(at, No{}, q);
-          } else {
+          const uint32_t in = kMode == kDistillGrad ? in_sum[at / kDisGroup] | kNone : ~0u;
+          if (in == ~0u && close && by_vectors && at + (kDisGroup - 1) * kCompute < c.wholes && !(c.cut && at == 0)) {
+            uint4 q[kDisGroup];
 #pragma unroll
-            for (int u = 0; u < kDisGroup; ++u)
-              if (at + u * kCompute < c.mine) q[u] = stage[tid + at + u * kCompute];
-          }
-#pragma unroll
-          for (int u = 0; u < kDisGroup; ++u) {
-            float y[kVec];
-            R::unpack(q[u], y);
-            if (close) {
-#pragma unroll
-              for (int k = 0; k < kVec; ++k) y[k] = exp2_approx(fmaf(y[k], log2e_t, offset));
-            } else {
-#pragma unroll
-              for (int k = 0; k < kVec; ++k) y[k] = exp2_approx((y[k] - rest_max) * log2e_t + shift);
-            }
-            if constexpr (sizeof(T) == 4) {
-#pragma unroll
-              for (int k = 0; k < kVec; ++k) y[k] *= size;
-            }
-            q[u] = R::pack(y);
-            if constexpr (sizeof(T) != 4) q[u] = make_uint4(q[u].x ^ sign, q[u].y ^ sign, q[u].z ^ sign, q[u].w ^ sign);
-            if (by_vectors && c.whole(at + u * kCompute)) to[at + u * kCompute] = q[u];
-          }
-          if (!by_vectors || c.any_partial()) {             // by way of the stage, where the vector is not needed any more
+            for (int u = 0; u < kDisGroup; ++u) q[u] = stage[tid + at + u * kCompute];
 #pragma unroll
             for (int u = 0; u < kDisGroup; ++u) {
-              const int i = at + u * kCompute, v = tid + i;
-              if (i >= c.mine || (by_vectors && c.whole(i))) continue;
-              stage[v] = q[u];
-              copy_ids<T>(grad, reinterpret_cast<const T *>(stage) + c.lead, max(0, v * kVec - c.lead), min(len, (v + 1) * kVec - c.lead));
+              float y[kVec];
+              R::unpack(q[u], y);
+#pragma unroll
+              for (int k = 0; k < kVec; ++k) y[k] = exp2_approx(fmaf(y[k], log2e_t, offset));
+              to[at + u * kCompute] = finish_vector(y);
+            }
+          } else {
+#pragma unroll 1
+            for (int u = 0; u < kDisGroup && at + u * kCompute < c.mine; ++u) {
+              float y[kVec];
+              R::unpack(take(at, u, in, false), y);
+#pragma unroll
+              for (int k = 0; k < kVec; ++k) y[k] = exp2_approx(fmaf(y[k], rest_scaled, rest_offset) * rest_factor + rest_shift);
+              const uint4 g = finish_vector(y);
+              const int v = tid + at + u * kCompute;
+              if (by_vectors && c.whole(at + u * kCompute)) {
+                to[at + u * kCompute] = g;
+              } else {                        // by way of the stage, where the vector is not needed any more
+                stage[v] = g;
+                copy_ids<T>(grad, reinterpret_cast<const T *>(stage) + c.lead, max(0, v * kVec - c.lead), min(len, (v + 1) * kVec - c.lead));
+              }
             }
           }
         };
@@ -568,15 +622,6 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
 #pragma unroll 1
               for (int k = max(0, (tid + i) * kVec - c.lead); k < min(len, (tid + i + 1) * kVec - c.lead); ++k) grad[k] = each;
             }
-          }
-        }
-        if (!fill) {
-          barrier_of<1, kCompute>();          // (zeros stand where listed ids are)
-          for (int e = tid; e < a.top; e += kCompute) {
-            const unsigned local = unsigned(ids[(turn & 1) * top_room + e]) - unsigned(begin);
-            if (local >= unsigned(len)) continue;
-            const float q = exp2_approx((zs[(turn & 1) * top_room + e] - largest) * p.log2e_t) * inverse_sum;
-            grad[local] = R::store(float(factor * (double(q) - weights[(turn & 1) * top_room + e] * inverse)));
           }
         }
       }

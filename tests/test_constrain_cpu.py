@@ -90,19 +90,25 @@ def test_team_kernels_read_between_barriers():
             head = "for (int turn = -1; turn <= turns; ++turn) {"
             loop = braced(body, body.index(head))
             behind = body[body.index(head) + len(head) + len(loop):]
-            assert behind.strip("}; \n").endswith("if (p.team > 1) team_barrier()") and not re.search(r"\b(?:return|break|continue);", without_lambdas(
-                loop.replace(braced(loop, loop.index("for (int e = tid; e < a.top")), "")))
+            assert behind.strip("}; \n").endswith("if (p.team > 1) team_barrier()") and not re.search(r"\b(?:return|break);", without_lambdas(loop))
             listing = braced(loop, loop.index("if (warp >= kWarps) {"))
-            assert re.findall(r"(if \([^)]*\)) team_(\w+)\(\);", listing) == [("if (together && has)", "arrive"), ("if (together && has)", "wait")]
-            assert listing.index("team_arrive") < listing.index("take_list") < listing.index("team_wait")
-            computing = loop.replace(listing, "")   # (its branch is the one with `has`)
-            assert "} else if (!has) {" in computing
-            assert re.findall(r"\bteam_(barrier|arrive|wait)\(", computing) == ["barrier"] and "if (together) team_barrier();" in computing
+            first = braced(loop, loop.index("} else if (!has) {"))
+            computing = loop[loop.index("} else if (!has) {") + len(first):]
+            calls = lambda text: re.findall(r"if \(([^()]*(?:\([^()]*\))?[^()]*)\) team_(\w+)\(\);|\bteam_(\w+)\(\);", text)  # noqa: E731
+            # every thread arrives once a turn that has a row, and waits once for it: in the same turn, or (the loss alone) in the next one
+            assert calls(listing) == [("together && turn > 0", "wait", ""), ("together && has", "arrive", ""),
+                                      ("kMode != kDistillLoss && together && has", "wait", "")]
+            assert re.search(r"if \(kMode == kDistillLoss\) \{\s*if \(together && turn > 0\) team_wait\(\);", listing)
+            assert calls(first) == [("kMode == kDistillLoss && together && turn > 0", "wait", "")]
+            assert re.sub(r"\s+", " ", computing[computing.index("if (kMode == kDistillLoss) { if".split(" if")[0], computing.index("float rest_max")):]
+                          ).startswith("if (kMode == kDistillLoss) { if (together) { if (turn > 0) team_wait(); team_arrive(); } } else if (together) { team_barrier(); }")
+            assert [c[1] or c[2] for c in calls(computing)] == ["wait", "arrive", "barrier"]
+            # the words that are read are written in front of the arrival, and again four turns on, when every reader has arrived for a later row
+            assert computing.index("s.sums[turn & 3][warp] = ") < computing.index("team_wait();")
+            assert len(TEAM_READ.findall(body)) == 1 and "team_read(&s.sums[turn & 3]" in braced(body, body.index("auto combine = "))
+            assert listing.index("team_wait();") < listing.index("combine(turn - 1)") < listing.index("team_arrive();")
+            assert computing.index("team_barrier();") < computing.index("combine(turn)") and body.count("combine(turn") == 2
             assert "const bool together = p.team > 1 && (kMode != kDistillGrad || p.in_place);" in body
-            assert len(TEAM_READ.findall(body)) == 1 and computing.index("team_barrier();") < TEAM_READ.search(computing).start()
-            # the words that are read are those of the turn's parity: written before the barrier, and again behind the next one
-            assert "s.sums[turn & 1][warp] = " in computing[:computing.index("team_barrier();")]
-            assert "team_read(&s.sums[turn & 1]" in computing
     assert seen == {"constrain_kernel", "distill_kernel"}
     users = {n for n in os.listdir(CSRC) if n.endswith((".cu", ".cuh")) and "team_rank()" in source(n)}
     assert users == {"constrain.cu", "distill.cu", "row_team.cuh"}
