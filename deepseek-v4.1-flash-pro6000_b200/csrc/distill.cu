@@ -12,74 +12,14 @@
 // asynchronous copy on (no barrier between copy and use), and where it has written a vector's gradient it starts the copy of the
 // next row's.  Two more warps are a row ahead: one gathers and reduces the next row's list, the other sets the bits of the ids
 // that count into the sum and, a row behind, takes the loss in FP64.  Three CTAs share an SM, each at another point of its row.
-#include "row_types.cuh"
+#include "distill_stream.cuh"
 #include "row_team.cuh"
 #include "host_error.h"
-#include "launch.h"
-#include <cfloat>
-#include <cmath>
 #include <type_traits>
 
 namespace ds41 {
 namespace {
 
-enum DistillMode { kDistillLoss, kDistillGrad, kDistillBoth };
-constexpr int kDisGroup = 4;                  // vectors of a thread that are copied, waited for and worked on together
-constexpr int kDisGroups = 5;                 // (the last for the one vector more of a slice that does not begin on a vector)
-constexpr int kDisVectors = kDisGroup * (kDisGroups - 1);
-constexpr int kDisTop = DS41_B200_DISTILL_MAX_TOP;
-constexpr int kDisOwn = kDisTop / 32;         // entries of a lane
-constexpr double kDisMost = 1.01;             // what a list's probabilities may add up to: 1, and the rounding of stored values
-
-struct DistillParams {
-  ds41_b200_distill_args a;
-  int in_place;                               // grad is logits
-  int slice, team;                            // ids of a CTA (a multiple of 32), CTAs of a row
-  float log2e_t;                              // log2(e) / T
-};
-
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void copies_wait(int left) {
-  switch (left) {
-    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-    case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-    default: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-  }
-}
-template <int kBarrier, int kCount> __device__ __forceinline__ void barrier_of() {
-  __syncwarp();
-  asm volatile("bar.sync %0, %1;" ::"n"(kBarrier), "n"(kCount) : "memory");
-}
-
-__device__ __forceinline__ float exp2_approx(float x) {   // 2 ulp; 0 for -inf and below 2^-126
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// An exponent of two below which, and above whose negative, a product of logit and log2(e) / T is taken as it is: the power of
-// x c - r with r = m c rounded is one fused multiply-add, its argument as exact as that of (x - m) c, if the rounding of r is made good for
-// once a row.  Beyond (rows of a type's lowest values) it is (x - m) c.
-constexpr float kDisNear = 1e37f;
-__device__ __forceinline__ bool near_exponent(float r) { return fabsf(r) < kDisNear; }
-__device__ __forceinline__ float excess(float m, float c, float r) { return near_exponent(r) ? fmaf(m, c, -r) : 0.f; }
-
-// Out of line, once each: what runs a few times a row shall not push the loops out of the instruction cache.
-__device__ __noinline__ double exp_of(double x) { return exp(x); }
-__device__ __noinline__ double log_of(double x) { return log(x); }
-__device__ __noinline__ double over(double x, double y) { return x / y; }
-
-// What is known of a row besides its ids outside the list, the same in every CTA of the team.
-struct DistillRow {
-  float scale;
-  int reject;                                 // of the list
-  float4 stats;                               // of the forward pass, in the gradient's
-  float zmax, share;                          // largest logit of the entries that count; sum of exp((z - zmax) / T), an entry per id
-  double kept, entropy, rest;                 // with w the unnormalised weights: sum of w, of w (ln w - (z - zmax) / T); 1 - the list's sum
-  double inverse, inverse_rest;               // 1 / (sum of w), 1 / (that + rest)
-};
 template <int kCompute>
 struct DistillSmem {
   DistillRow rows[4];                         // by the number of the row's turn: the last one, this one, the next two
@@ -87,35 +27,6 @@ struct DistillSmem {
   float2 result[2];                           // (maximum, sum) of the row's ids outside the list
   float2 all[2];                              // of all its ids: the maximum, 1 / the sum; a NaN where the gradient has no listed ids to set
 };
-
-// A row's slice as one of its CTA's threads sees it, which takes vectors t, t + kCompute, ... of it ("at" 0, kCompute, ...).  Place 0 is
-// where the vector of the slice's first id begins.
-template <class T, int kCompute>
-struct DistillSlice {
-  static constexpr int kVec = RowType<T>::kVec;
-  const T *x;
-  const uint4 *from;                          // the thread's first vector
-  int lead, vecs;                             // vectors of the slice
-  int mine, wholes;                           // its vectors are the slice's below `mine`, and hold no other slice's ids below `wholes`
-  bool cut;                                   // ... but for the first one
-  __device__ __forceinline__ DistillSlice(const DistillParams &p, int row, int begin, int len, int t) {
-    x = static_cast<const T *>(p.a.logits) + size_t(row) * size_t(p.a.logits_stride) + begin;
-    lead = int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % kVec);
-    vecs = (lead + len + kVec - 1) / kVec;
-    from = reinterpret_cast<const uint4 *>(x - lead) + t;
-    mine = vecs - t; wholes = (lead + len) / kVec - t;
-    cut = lead && t == 0;
-  }
-  __device__ __forceinline__ bool whole(int at) const { return at < wholes && !(cut && at == 0); }
-  __device__ __forceinline__ bool any_partial() const { return cut || wholes < mine; }
-};
-
-// A vector that is not whole comes and goes by its ids, `from` .. `to`.
-template <class T>
-__device__ __noinline__ void copy_ids(T *to_first, const T *from_first, int from, int to) {
-#pragma unroll 1
-  for (int i = from; i < to; ++i) to_first[i] = from_first[i];
-}
 
 // Words of bits for a slice of so many bytes.
 template <int kCompute> __host__ __device__ __forceinline__ int distill_bit_words(int bytes) {
@@ -143,12 +54,9 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
   uint32_t *const mask_words = bits + 2 * bits_room;   // of the slice, as they come
   auto bit_word = [](int v) { return v / (kDisGroup * kCompute) * kCompute + v % kCompute; };
   auto bit_shift = [](int v) { return v / kCompute % kDisGroup * kVec; };
-  const double t = a.temperature;
   cudaGridDependencySynchronize();
   cudaTriggerProgrammaticLaunchCompletion();
 
-  auto row_scale = [&](int row) { return kMode != kDistillLoss && a.row_scale && row < a.rows ? load_input(a.row_scale + row) : 1.f; };
-  auto skipped = [&](const DistillRow &r) { return kMode != kDistillLoss && r.scale == 0.f; };
   // the copies of a group of the thread's vectors
   auto start_copies = [&](const DistillSlice<T, kCompute> &c, int at) {
     const uint32_t to = uint32_t(__cvta_generic_to_shared(stage + tid + at));
@@ -168,123 +76,16 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
   };
 
   // ---- the list of the row of turn `turn`, by one warp
+  auto list_of = [&](int turn) { return DistillList{weights + (turn & 1) * top_room, ids + (turn & 1) * top_room, zs + (turn & 1) * top_room}; };
   auto take_list = [&](int row, int turn) {
-    DistillRow &r = s.rows[turn & 3];
-    double *const w_list = weights + (turn & 1) * top_room;
-    int *const id_list = ids + (turn & 1) * top_room;
-    float *const z_list = zs + (turn & 1) * top_room;
-    const T *whole = static_cast<const T *>(a.logits) + size_t(row) * size_t(a.logits_stride);
-    const uint32_t *mask = a.mask ? a.mask + size_t(row) * size_t(a.mask_stride) : nullptr;
-    const int own = (a.top + 31) / 32;
-    unsigned named = 0u, counts = 0u;         // a bit per entry of the lane
-    bool bad = false;
-    float most = -FLT_MAX, zmax = -FLT_MAX;
-#pragma unroll 1
-    for (int k = 0; k < own; ++k) {
-      const int e = lane + 32 * k;
-      int id = -1;
-      double value = 0.0;
-      float z = 0.f;
-      if (e < a.top) {
-        id = load_input(a.teacher_ids + size_t(row) * size_t(a.ids_stride) + e);
-        const size_t at = size_t(row) * size_t(a.values_stride) + e;
-        value = a.teacher_dtype == DS41_B200_F64 ? load_input(static_cast<const double *>(a.teacher_values) + at)
-                                                 : double(load_input(static_cast<const float *>(a.teacher_values) + at));
-      }
-      if (id >= 0 && id < a.vocab) {
-        named |= 1u << k;
-        bad |= !(value < INFINITY);
-        if (!mask || ((load_input(mask + (id >> 5)) >> (id & 31)) & 1u)) {
-          z = R::load(whole[id]);
-          bad |= !(z < INFINITY);
-          if (!(z == -INFINITY)) { counts |= 1u << k; most = fmaxf(most, float(value)); zmax = fmaxf(zmax, z); }
-        }
-      }
-      if (e < top_room) { id_list[e] = (counts >> k) & 1u ? id : -2 - e; w_list[e] = value; z_list[e] = z; }
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      zmax = fmaxf(zmax, __shfl_xor_sync(0xffffffffu, zmax, o));
-    }
-    __syncwarp();
-    unsigned first = counts;                  // entries with no other of the same id in front of them
-#pragma unroll 1
-    for (int k = 0; k < own; ++k) {
-      if (!((counts >> k) & 1u)) continue;
-      const int e = lane + 32 * k, id = id_list[e];
-#pragma unroll 2
-      for (int j = 0; 4 * j < e; ++j) {
-        const int4 q = reinterpret_cast<const int4 *>(id_list)[j];
-        const int before = e - 4 * j;
-        if (q.x == id || (before > 1 && q.y == id) || (before > 2 && q.z == id) || (before > 3 && q.w == id)) { first &= ~(1u << k); break; }
-      }
-    }
-    const bool again = __any_sync(0xffffffffu, first != counts);
-    double list = 0.0, kept = 0.0, entropy = 0.0;
-    float share = 0.f;
-#pragma unroll 1
-    for (int k = 0; k < own; ++k) {
-      const int e = lane + 32 * k;
-      if (!((named >> k) & 1u)) continue;
-      const double log_w = a.tail ? w_list[e] : over(w_list[e] - double(most), t), w = exp_of(log_w);
-      list += w;
-      const bool is = (counts >> k) & 1u;
-      w_list[e] = is ? w : 0.0;
-      if (!is) continue;
-      kept += w;
-      if (!again) {
-        const double gap = over(double(z_list[e]) - double(zmax), t);
-        if (w > 0.0) entropy += w * (log_w - gap);
-        share += exp2_approx((z_list[e] - zmax) * p.log2e_t);
-      }
-    }
-    if (again) {                              // an id's first entry takes the weights of the later ones
-      __syncwarp();
-      double merged[kDisOwn];
-#pragma unroll 1
-    for (int k = 0; k < own; ++k) {
-        const int e = lane + 32 * k;
-        merged[k] = e < a.top ? w_list[e] : 0.0;
-        if (!((first >> k) & 1u)) continue;
-#pragma unroll 1
-        for (int j = e + 1; j < a.top; ++j)
-          if (id_list[j] == id_list[e]) merged[k] += w_list[j];
-        const double gap = over(double(z_list[e]) - double(zmax), t);
-        if (merged[k] > 0.0) entropy += merged[k] * (log_of(merged[k]) - gap);
-        share += exp2_approx((z_list[e] - zmax) * p.log2e_t);
-      }
-      __syncwarp();
-#pragma unroll 1
-    for (int k = 0; k < own; ++k) {
-        const int e = lane + 32 * k;
-        if (e >= a.top) continue;
-        w_list[e] = merged[k];
-        if (((counts & ~first) >> k) & 1u) id_list[e] = -2 - e;
-      }
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      list += __shfl_xor_sync(0xffffffffu, list, o);
-      kept += __shfl_xor_sync(0xffffffffu, kept, o);
-      entropy += __shfl_xor_sync(0xffffffffu, entropy, o);
-      share += __shfl_xor_sync(0xffffffffu, share, o);
-    }
-    bad = __any_sync(0xffffffffu, bad);
-    if (lane == 0) {
-      r.reject = bad ? DS41_B200_ROW_NONFINITE : a.tail && list > kDisMost ? DS41_B200_ROW_NOT_NORMALIZED : !(kept > 0.0) ? DS41_B200_ROW_EMPTY : 0;
-      r.zmax = zmax; r.share = share; r.kept = kept; r.entropy = entropy;
-      r.rest = a.tail ? fmax(0.0, 1.0 - list) : 0.0;
-      r.inverse = over(1.0, kept); r.inverse_rest = over(1.0, kept + r.rest);
-      if (kMode == kDistillGrad) r.stats = reinterpret_cast<const float4 *>(a.stats)[row];
-    }
+    const DistillList list = list_of(turn);
+    gather_list<T, kMode>(p, row, s.rows[turn & 3], list, lane);
     barrier_of<2, 64>();                      // (the bits are set)
     const DistillSlice<T, kCompute> c(p, row, begin, len, 0);
     uint32_t *const out = bits + (turn & 1) * bits_room;
 #pragma unroll 1
-    for (int k = 0; k < own; ++k) {
-      const int e = lane + 32 * k;
-      const unsigned local = e < a.top ? unsigned(id_list[e]) - unsigned(begin) : ~0u;
+    for (int e = lane; e < a.top; e += 32) {
+      const unsigned local = unsigned(list.ids[e]) - unsigned(begin);
       if (local < unsigned(len)) {
         const int place = int(local) + c.lead, v = place / kVec;
         atomicAnd(&out[bit_word(v)], ~(1u << (bit_shift(v) + place % kVec)));
@@ -329,35 +130,6 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
     }
     barrier_of<2, 64>();
   };
-  // ---- loss, stats and status of a row that is done
-  auto finish = [&](int row, int turn) {
-    const DistillRow &r = s.rows[turn & 3];
-    if (skipped(r)) {
-      a.loss[row] = 0.f; a.status[row] = 0;
-      if (a.stats) reinterpret_cast<float4 *>(a.stats)[row] = make_float4(0.f, 0.f, 0.f, 0.f);
-      return;
-    }
-    const float rest_max = s.result[turn & 1].x, rest_sum = s.result[turn & 1].y, nan = __int_as_float(0x7fffffff);
-    const int reject = r.reject ? r.reject : rest_sum < INFINITY ? 0 : DS41_B200_ROW_NONFINITE;
-    float loss = reject == DS41_B200_ROW_EMPTY ? 0.f : nan;
-    float4 stats = make_float4(nan, nan, nan, nan);
-    if (!reject) {
-      const bool any = rest_sum != 0.f;
-      const double zmax = r.zmax, largest = any ? fmax(double(rest_max), zmax) : zmax;
-      const double down = any ? over(double(rest_max) - largest, t) : 0.0, list_down = over(zmax - largest, t);
-      const double log_rest = log_of(double(rest_sum));
-      const double log_sum = log_of((any ? double(rest_sum) * exp_of(down) : 0.0) + double(r.share) * exp_of(list_down));
-      const double inverse = any ? r.inverse_rest : r.inverse, kept = r.kept * inverse, tail = any ? r.rest * inverse : 0.0;
-      double sum = r.entropy * inverse + kept * (log_of(inverse) + log_sum - list_down);
-      if (tail > 0.0) sum += tail * (log_of(tail) - (down + log_rest - log_sum));
-      loss = float(t * t * sum);
-      stats = make_float4(float(largest), float(log_sum), any ? rest_max : -INFINITY, any ? float(log_rest) : -INFINITY);
-    }
-    a.loss[row] = loss;
-    a.status[row] = reject;
-    if (a.stats) reinterpret_cast<float4 *>(a.stats)[row] = stats;
-  };
-
   // (maximum, sum) of the ids outside the list of the turn's row, from the whole team's warps: 64 at most, in the same order everywhere
   auto combine = [&](int turn) {
     float most = -FLT_MAX, sum = 0.f;
@@ -375,23 +147,6 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return make_float2(all, sum);
   };
-  // ---- the gradient of the listed ids of a row whose other ids are written
-  auto set_listed = [&](int row, int turn) {
-    const DistillRow &r = s.rows[turn & 3];
-    const float2 all = s.all[turn & 1];
-    if (!(all.y == all.y)) return;
-    const double inverse = s.result[turn & 1].y != 0.f ? r.inverse_rest : r.inverse, factor = double(r.scale) * t;
-    T *const grad = static_cast<T *>(a.grad) + size_t(row) * size_t(a.grad_stride) + begin;
-#pragma unroll 1
-    for (int e = lane; e < a.top; e += 32) {
-      const unsigned local = unsigned(ids[(turn & 1) * top_room + e]) - unsigned(begin);
-      if (local >= unsigned(len)) continue;
-      const float q = exp2_approx((zs[(turn & 1) * top_room + e] - all.x) * p.log2e_t) * all.y;
-      grad[local] = R::store(float(factor * (double(q) - weights[(turn & 1) * top_room + e] * inverse)));
-    }
-    __syncwarp();                             // (the list's memory is the next but one row's)
-  };
-
   // The team's CTAs wait for one another once a row: for each other's sums, and until each has read of the row what it needs of other
   // slices.  The loss alone is not waited for by the compute warps until they have the next row's sums.
   const bool together = p.team > 1 && (kMode != kDistillGrad || p.in_place);
@@ -410,18 +165,18 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
       }
       if (together && has) team_arrive();
       if (warp == kWarps) {
-        if (kMode != kDistillLoss && turn > 0) set_listed(row - teams, turn - 1);
+        if (kMode != kDistillLoss && turn > 0) set_listed<T>(p, row - teams, s.rows[(turn - 1) & 3], list_of(turn - 1), s.result[(turn - 1) & 1], s.all[(turn - 1) & 1], begin, len, lane);
         if (has_next) take_list(next, turn + 1);
       } else {
-        if (lane == 0) s.rows[(turn + 2) & 3].scale = row_scale(next + teams);
-        if (lane == 0 && turn < 0) s.rows[0].scale = row_scale(next);
+        if (lane == 0) s.rows[(turn + 2) & 3].scale = row_scale_of<kMode>(p, next + teams);
+        if (lane == 0 && turn < 0) s.rows[0].scale = row_scale_of<kMode>(p, next);
         if (has_next) take_bits(next, turn + 1);
-        if (kMode != kDistillGrad && rank == 0 && lane == 0 && turn > 0) finish(row - teams, turn - 1);
+        if (kMode != kDistillGrad && rank == 0 && lane == 0 && turn > 0) finish_row<kMode>(p, row - teams, s.rows[(turn - 1) & 3], s.result[(turn - 1) & 1]);
       }
       if (kMode != kDistillLoss && together && has) team_wait();
     } else if (!has) {
       if (kMode == kDistillLoss && together && turn > 0) team_wait();
-      if (has_next && row_scale(next) != 0.f) {
+      if (has_next && row_scale_of<kMode>(p, next) != 0.f) {
         const DistillSlice<T, kCompute> c(p, next, begin, len, tid);
 #pragma unroll 1
         for (int g = 0; g < kDisGroups; ++g) start_copies(c, g * kDisGroup * kCompute);
@@ -429,7 +184,7 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
     } else {
       const DistillRow &r = s.rows[turn & 3];
       const DistillSlice<T, kCompute> c(p, row, begin, len, tid), c_next(p, has_next ? next : row, begin, len, tid);
-      const bool skip = skipped(r), ahead = has_next && !skipped(s.rows[(turn + 1) & 3]);
+      const bool skip = skipped<kMode>(r), ahead = has_next && !skipped<kMode>(s.rows[(turn + 1) & 3]);
       const uint32_t *const in_sum = bits + (turn & 1) * bits_room + tid;
       const float log2e_t = p.log2e_t;
       T *const grad = kMode == kDistillLoss ? nullptr : static_cast<T *>(a.grad) + size_t(row) * size_t(a.grad_stride) + begin;
@@ -532,52 +287,25 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
 
       // ---- the gradient
       if (kMode != kDistillLoss) {
-        float largest, inverse_sum, q_rest;   // of all ids: the maximum, 1 / the sum; share of the ids outside the list
-        bool any;
-        int reject = r.reject;
-        if (kMode == kDistillGrad) {
-          largest = r.stats.x; inverse_sum = exp2_approx(-r.stats.y * 1.44269504f);
-          any = r.stats.w > -INFINITY;
-          rest_max = any ? r.stats.z : 0.f;
-          rest_sum = any ? exp2_approx(r.stats.w * 1.44269504f) : 0.f;
-          q_rest = any ? rest_sum * exp2_approx((rest_max - largest) * p.log2e_t) * inverse_sum : 0.f;
-          if (!reject && !(r.stats.x == r.stats.x)) reject = DS41_B200_ROW_NONFINITE;
-        } else {
-          any = rest_sum != 0.f;
-          largest = any ? fmaxf(rest_max, r.zmax) : r.zmax;
-          const float part = any ? rest_sum * exp2_approx((rest_max - largest) * p.log2e_t) : 0.f;
-          inverse_sum = 1.f / (part + r.share * exp2_approx((r.zmax - largest) * p.log2e_t));
-          q_rest = part * inverse_sum;
-          if (!reject && !(rest_sum < INFINITY)) reject = DS41_B200_ROW_NONFINITE;
-        }
-        const float tail = any ? float(r.rest * r.inverse_rest) : 0.f, coef = any ? r.scale * float(t) * (q_rest - tail) / rest_sum : 0.f;
-        const bool fill = skip || reject != 0;
+        const DistillFactors f = gradient_factors<kMode, sizeof(T)>(p, r, rest_max, rest_sum);
+        const bool fill = skip || f.reject != 0;
         if (tid == 0) {
-          s.result[turn & 1] = make_float2(rest_max, rest_sum);
-          s.all[turn & 1] = make_float2(largest, fill ? __int_as_float(0x7fffffff) : inverse_sum);
+          s.result[turn & 1] = make_float2(f.rest_max, f.rest_sum);
+          s.all[turn & 1] = make_float2(f.largest, fill ? __int_as_float(0x7fffffff) : f.inverse_sum);
         }
-        // 16-bit types: the factor's size goes into the exponent, its sign into the words (exponents below 256 are off by 2^-17, a power
-        // by 2^-17, which is little beside the rounding to 16 bits)
-        const float rest_c = rest_max * log2e_t;
-        const bool close = sizeof(T) == 4 ? near_exponent(rest_c) : fabsf(rest_c) < 256.f;
-        const float shift = sizeof(T) == 4 ? 0.f : log2f(fabsf(coef)), size = sizeof(T) == 4 ? coef * exp2_approx(-excess(rest_max, log2e_t, rest_c)) : 1.f;
-        const float offset = sizeof(T) == 4 ? -rest_c : shift - rest_c - excess(rest_max, log2e_t, rest_c);
-        const uint32_t sign = sizeof(T) != 4 && coef < 0.f ? 0x80008000u : 0u;
         uint4 *const to = reinterpret_cast<uint4 *>(grad - c.lead) + tid;
-        const float rest_scaled = close ? log2e_t : 1.f, rest_factor = close ? 1.f : log2e_t;
-        const float rest_offset = close ? offset : -rest_max, rest_shift = close ? 0.f : shift;
         auto finish_vector = [&](float (&y)[kVec]) {
           if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int k = 0; k < kVec; ++k) y[k] *= size;
+            for (int k = 0; k < kVec; ++k) y[k] *= f.size;
           }
           uint4 g = R::pack(y);
-          if constexpr (sizeof(T) != 4) g = make_uint4(g.x ^ sign, g.y ^ sign, g.z ^ sign, g.w ^ sign);
+          if constexpr (sizeof(T) != 4) g = make_uint4(g.x ^ f.sign, g.y ^ f.sign, g.z ^ f.sign, g.w ^ f.sign);
           return g;
         };
         auto step = [&](int at) {
           const uint32_t in = kMode == kDistillGrad ? in_sum[at / kDisGroup] | kNone : ~0u;
-          if (in == ~0u && close && by_vectors && at + (kDisGroup - 1) * kCompute < c.wholes && !(c.cut && at == 0)) {
+          if (in == ~0u && f.close && by_vectors && at + (kDisGroup - 1) * kCompute < c.wholes && !(c.cut && at == 0)) {
             uint4 q[kDisGroup];
 #pragma unroll
             for (int u = 0; u < kDisGroup; ++u) q[u] = stage[tid + at + u * kCompute];
@@ -586,7 +314,7 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
               float y[kVec];
               R::unpack(q[u], y);
 #pragma unroll
-              for (int k = 0; k < kVec; ++k) y[k] = exp2_approx(fmaf(y[k], log2e_t, offset));
+              for (int k = 0; k < kVec; ++k) y[k] = exp2_approx(fmaf(y[k], log2e_t, f.offset));
               to[at + u * kCompute] = finish_vector(y);
             }
           } else {
@@ -595,7 +323,7 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
               float y[kVec];
               R::unpack(take(at, u, in, false), y);
 #pragma unroll
-              for (int k = 0; k < kVec; ++k) y[k] = exp2_approx(fmaf(y[k], rest_scaled, rest_offset) * rest_factor + rest_shift);
+              for (int k = 0; k < kVec; ++k) y[k] = exp2_approx(fmaf(y[k], f.scaled, f.minus) * f.factor + f.shift);
               const uint4 g = finish_vector(y);
               const int v = tid + at + u * kCompute;
               if (by_vectors && c.whole(at + u * kCompute)) {
@@ -612,7 +340,7 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
         } else {                              // (a row that was rejected, or is padding)
           if (!skip) copies_wait(0);
           run(No{}, Yes{}, [](int) {});
-          const T each = !skip && reject != DS41_B200_ROW_EMPTY ? R::store(__int_as_float(0x7fffffff)) : R::store(0.f);
+          const T each = !skip && f.reject != DS41_B200_ROW_EMPTY ? R::store(__int_as_float(0x7fffffff)) : R::store(0.f);
           const T pair[2] = {each, each};
           const uint32_t w = sizeof(T) == 4 ? *reinterpret_cast<const uint32_t *>(&each) : *reinterpret_cast<const uint32_t *>(pair);
 #pragma unroll 1
@@ -630,6 +358,9 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
   }
   if (p.team > 1) team_barrier();
 }
+
+constexpr int kStreamRows = 148;
+constexpr int kStreamSmem = 111 * 1024;       // two CTAs an SM
 
 // Teams that the GPU holds at a time (asked of the runtime once per variant, device, team and shared memory of a thread's calls).
 template <class T, int kMode, int kCompute>
@@ -679,7 +410,29 @@ cudaError_t launch_distill(const DistillParams &p, cudaStream_t stream) {
 }
 
 template <class T, int kMode>
+cudaError_t launch_stream(const DistillParams &p, size_t smem, cudaStream_t stream) {
+  static thread_local struct { int dev, ctas; size_t smem; } known{-1, 0, 0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (known.dev != dev || known.smem != smem) {
+    int per_sm = 0, sms = 0;
+    e = cudaFuncSetAttribute(distill_stream_kernel<T, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamSmem);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, distill_stream_kernel<T, kMode>, kStreamThreads + 64, smem);
+    if (e != cudaSuccess) return e;
+    known = {dev, per_sm * sms < 1 ? 1 : per_sm * sms, smem};
+  }
+  const int turns = (p.a.rows + known.ctas - 1) / known.ctas;
+  return launch_early(distill_stream_kernel<T, kMode>, (p.a.rows + turns - 1) / turns, kStreamThreads + 64, smem, stream, p);
+}
+
+template <class T, int kMode>
 cudaError_t launch_distill(DistillParams &d, cudaStream_t stream) {
+  // Long rows, and enough of them for one CTA each
+  d.groups = stream_groups(d.a.vocab, RowType<T>::kVec);
+  const size_t smem = size_t(kStreamRing) * kDisGroup * kStreamThreads * 16 + 2 * size_t((d.a.top + 3) & ~3) * 16 + 2 * size_t(stream_marks<T>(d.groups));
+  if (!d.a.mask && d.a.top < 256 && d.groups >= kStreamRing && d.a.rows >= kStreamRows && smem <= kStreamSmem) return launch_stream<T, kMode>(d, smem, stream);
   constexpr int kSmall = 64 * kDisVectors * 16 / int(sizeof(T)), kLarge = 4 * kSmall;   // ids of a CTA
   const int vocab = d.a.vocab;
   // CTAs per row: as few as hold it, three CTAs to an SM where eight of them can, and for batches that leave SMs idle up to eight, of at least
@@ -720,7 +473,7 @@ int distill(const ds41_b200_distill_args *p, cudaStream_t stream) {
     if (!rows_apart_or_same(p->logits, p->logits_stride, p->grad, p->grad_stride, p->rows, p->vocab, bytes))
       return invalid("distill args: grad overlaps logits without being the same rows");
   }
-  DistillParams d{*p, p->grad == p->logits, 0, 1, float(1.4426950408889634 / p->temperature)};
+  DistillParams d{*p, p->grad == p->logits, 0, 1, 0, float(1.4426950408889634 / p->temperature)};
   switch (p->dtype) {
     case DS41_B200_F32: return int(launch_distill<float, kMode>(d, stream));
     case DS41_B200_BF16: return int(launch_distill<__nv_bfloat16, kMode>(d, stream));

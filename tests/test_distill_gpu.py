@@ -18,12 +18,12 @@ def pkg():
     return entry.load_package()
 
 
-def check(pkg, c, dtype, temperature=1.0, tail=False, lead=0, gap=0, out_lead=0, out_gap=0):
+def check(pkg, c, dtype, temperature=1.0, tail=False, lead=0, gap=0, out_lead=0, out_gap=0, wants=None):
     rows, vocab = c["z"].shape
     view, buf, t = gpu(c, dtype, lead, gap)
     kept = buf.clone()
     more = {"temperature": temperature, "tail": tail, "mask": t["mask"]}
-    want, plain = want_of(c, temperature, tail), want_of(c, temperature, tail, scaled=False)
+    want, plain = wants or (want_of(c, temperature, tail), want_of(c, temperature, tail, scaled=False))
     grads = torch.full((rows, out_lead + vocab + out_gap), 5.0, dtype=dtype, device="cuda")
     out = grads[:, out_lead: out_lead + vocab]
 
@@ -111,6 +111,37 @@ def test_lists_and_rows_where_it_can_go_wrong(pkg, dtype, tail, temperature, voc
         assert want[3][12] == {900: -10, 70001: 0}[vocab]
     check(pkg, c, t, temperature, tail)
     check(pkg, c, t, temperature, tail, 1, 2, 1, 2)
+
+
+@pytest.mark.parametrize("dtype,vocab,tail,temperature", [("fp32", 50021, True, 1.0), ("fp32", 131072, False, 0.6), ("bf16", 50021, False, 1.7),
+                                                          ("bf16", 129280, True, 1.0), ("fp16", 50024, True, 1.0), ("fp16", 98305, False, 3.0)])
+def test_many_rows_where_it_can_go_wrong(pkg, dtype, vocab, tail, temperature):
+    """Batches of long rows that each CTA takes several of: rows to skip, to reject and to take, in every order, at every alignment."""
+    t = TYPES[dtype]
+    c = case(21, 16, vocab, t, 30, tail, teacher=np.float64)
+    inside = [np.setdiff1d(np.arange(vocab), c["ids"][r]) for r in range(16)]
+    c["scale"][:] = np.linspace(0.5, 1.5, 16)
+    c["scale"][[0, 5]] = 0.0
+    c["z"][0] = np.nan                                                    # padding rows are not read
+    c["z"][2, inside[2][-1]] = np.nan
+    c["z"][3, inside[3][0]] = np.inf
+    c["z"][4, inside[4][::2]] = -np.inf                                   # half of the ids are not allowed
+    c["z"][6, c["ids"][6, 1]] = -np.inf
+    c["ids"][7] = -1
+    c["values"][8, 2] = np.nan
+    c["ids"][9, 3:20] = c["ids"][9, 1]                                    # one id eighteen times
+    c["ids"][10] = np.arange(30)                                          # ids side by side, at the row's beginning and end
+    c["ids"][11] = vocab - 1 - np.arange(30)
+    c["z"][12] = torch.finfo(t).min
+    c["z"][13] = torch.finfo(t).min
+    c["z"][13, c["ids"][13]] = 1.0
+    c["scale"][14] = -1.0
+    times, order = 45, np.random.default_rng(22).permutation(16 * 45)
+    wants = [tuple(np.tile(w, (times,) + (1,) * (w.ndim - 1))[order] for w in want_of(c, temperature, tail, scaled)) for scaled in (True, False)]
+    assert wants[0][3][np.argsort(order)][:16].tolist() == [0, 0, -1, -1, 0, 0, 0, -2, -1, 0, 0, 0, 0, 0, 0, 0]
+    c = {k: np.tile(v, (times,) + (1,) * (v.ndim - 1))[order] for k, v in c.items()}
+    check(pkg, c, t, temperature, tail, wants=wants)
+    check(pkg, c, t, temperature, tail, 3, 2, 1, 0, wants=wants)          # (an output at another alignment)
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
