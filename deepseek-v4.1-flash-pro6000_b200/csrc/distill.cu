@@ -202,20 +202,36 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
       };
       using Yes = std::true_type;
       using No = std::false_type;
-      // one vector of a group whose bits are `in`, ids that are not in the sum as -inf; keep: in the stage too
-      auto take = [&](int at, int u, uint32_t in, bool keep) {
-        uint4 *const here = stage + tid + at + u * kCompute;
-        const unsigned some = (in >> (u * kVec)) & kAll;
-        if (some == kAll) return *here;
-        const uint4 q = R::only(*here, some);
-        if (keep) *here = q;
-        return q;
-      };
       constexpr uint32_t kNone = sizeof(T) == 4 ? 0xffff0000u : 0u;     // (a word's bits that are no vector's)
+      // the thread's vectors of a group, ids that are not in the sum as -inf; keep: in the stage too
+      auto take = [&](int at, bool keep, uint4 (&q)[kDisGroup]) {
+        uint4 *const here = stage + tid + at;
+        if (at + (kDisGroup - 1) * kCompute < c.mine) {
+#pragma unroll
+          for (int u = 0; u < kDisGroup; ++u) q[u] = here[u * kCompute];
+        } else {
+#pragma unroll
+          for (int u = 0; u < kDisGroup; ++u) {
+            q[u] = R::nothing();
+            if (at + u * kCompute < c.mine) q[u] = here[u * kCompute];
+          }
+        }
+        const uint32_t in = in_sum[at / kDisGroup] | kNone;
+        if (in != ~0u) {
+#pragma unroll
+          for (int u = 0; u < kDisGroup; ++u) {
+            q[u] = R::only(q[u], in >> (u * kVec));
+            if (keep && at + u * kCompute < c.mine) here[u * kCompute] = q[u];
+          }
+        }
+      };
 
       // ---- maximum and sum of the ids outside the list
       float high = -FLT_MAX, high_c = -INFINITY, sums[4] = {0.f, 0.f, 0.f, 0.f};   // (relative to high_c)
-      auto raise = [&](float top) {
+      auto add = [&](int at) {
+        uint4 q[kDisGroup];
+        take(at, kMode == kDistillBoth, q);
+        const float top = R::largest(q);
         if (top > high) {
           const float top_c = top * log2e_t;
           const float down = exp2_approx(near_exponent(top_c) && near_exponent(high_c) ? high_c - top_c : (high - top) * log2e_t);
@@ -223,37 +239,18 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
           for (int i = 0; i < 4; ++i) sums[i] *= down;
           high = top; high_c = top_c;
         }
-      };
-      auto add = [&](int at) {
-        const uint32_t in = in_sum[at / kDisGroup] | kNone;
-        bool fast = in == ~0u && at + (kDisGroup - 1) * kCompute < c.mine;
-        if (fast) {
-          uint4 q[kDisGroup];
+        const bool is_near = near_exponent(high_c);
+        const float scaled = is_near ? log2e_t : 1.f, minus = is_near ? -high_c : -high;
 #pragma unroll
-          for (int u = 0; u < kDisGroup; ++u) q[u] = stage[tid + at + u * kCompute];
-          raise(R::largest(q));
-          fast = near_exponent(high_c);
-          if (fast) {
+        for (int u = 0; u < kDisGroup; ++u) {
+          float y[kVec];
+          R::unpack(q[u], y);
+          if (is_near) {
 #pragma unroll
-            for (int u = 0; u < kDisGroup; ++u) {
-              float y[kVec];
-              R::unpack(q[u], y);
+            for (int k = 0; k < kVec; ++k) sums[k % 4] += exp2_approx(fmaf(y[k], scaled, minus));
+          } else {
 #pragma unroll
-              for (int k = 0; k < kVec; ++k) sums[k % 4] += exp2_approx(fmaf(y[k], log2e_t, -high_c));
-            }
-          }
-        }
-        if (!fast) {                          // some ids of the group are out, or not there, or far from the others
-#pragma unroll 1
-          for (int u = 0; u < kDisGroup && at + u * kCompute < c.mine; ++u) {
-            const uint4 q[1] = {take(at, u, in, kMode == kDistillBoth)};
-            raise(R::largest(q));
-            float y[kVec];
-            R::unpack(q[0], y);
-            const float factor = near_exponent(high_c) ? 1.f : log2e_t, scaled = near_exponent(high_c) ? log2e_t : 1.f;
-            const float minus = near_exponent(high_c) ? -high_c : -high;
-#pragma unroll
-            for (int k = 0; k < kVec; ++k) sums[k % 4] += exp2_approx(fmaf(y[k], scaled, minus) * factor);
+            for (int k = 0; k < kVec; ++k) sums[k % 4] += exp2_approx(fmaf(y[k], scaled, minus) * log2e_t);
           }
         }
       };
@@ -304,34 +301,37 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
           return g;
         };
         auto step = [&](int at) {
-          const uint32_t in = kMode == kDistillGrad ? in_sum[at / kDisGroup] | kNone : ~0u;
-          if (in == ~0u && f.close && by_vectors && at + (kDisGroup - 1) * kCompute < c.wholes && !(c.cut && at == 0)) {
-            uint4 q[kDisGroup];
+          uint4 q[kDisGroup];
+          if (kMode == kDistillGrad) {
+            take(at, false, q);
+          } else {
 #pragma unroll
-            for (int u = 0; u < kDisGroup; ++u) q[u] = stage[tid + at + u * kCompute];
+            for (int u = 0; u < kDisGroup; ++u)
+              if (at + u * kCompute < c.mine) q[u] = stage[tid + at + u * kCompute];
+          }
 #pragma unroll
-            for (int u = 0; u < kDisGroup; ++u) {
-              float y[kVec];
-              R::unpack(q[u], y);
+          for (int u = 0; u < kDisGroup; ++u) {
+            float y[kVec];
+            R::unpack(q[u], y);
+            if (f.close) {
 #pragma unroll
               for (int k = 0; k < kVec; ++k) y[k] = exp2_approx(fmaf(y[k], log2e_t, f.offset));
-              to[at + u * kCompute] = finish_vector(y);
-            }
-          } else {
-#pragma unroll 1
-            for (int u = 0; u < kDisGroup && at + u * kCompute < c.mine; ++u) {
-              float y[kVec];
-              R::unpack(take(at, u, in, false), y);
+            } else {
 #pragma unroll
               for (int k = 0; k < kVec; ++k) y[k] = exp2_approx(fmaf(y[k], f.scaled, f.minus) * f.factor + f.shift);
-              const uint4 g = finish_vector(y);
-              const int v = tid + at + u * kCompute;
-              if (by_vectors && c.whole(at + u * kCompute)) {
-                to[at + u * kCompute] = g;
-              } else {                        // by way of the stage, where the vector is not needed any more
-                stage[v] = g;
-                copy_ids<T>(grad, reinterpret_cast<const T *>(stage) + c.lead, max(0, v * kVec - c.lead), min(len, (v + 1) * kVec - c.lead));
-              }
+            }
+            q[u] = finish_vector(y);
+            if (by_vectors && c.whole(at + u * kCompute)) to[at + u * kCompute] = q[u];
+          }
+          if (!by_vectors || c.any_partial()) {   // by way of the stage, where the vectors are not needed any more
+#pragma unroll
+            for (int u = 0; u < kDisGroup; ++u)
+              if (at + u * kCompute < c.mine) stage[tid + at + u * kCompute] = q[u];
+#pragma unroll 1
+            for (int i = at; i < min(c.mine, at + kDisGroup * kCompute); i += kCompute) {
+              if (by_vectors && c.whole(i)) continue;
+              const int v = tid + i;
+              copy_ids<T>(grad, reinterpret_cast<const T *>(stage) + c.lead, max(0, v * kVec - c.lead), min(len, (v + 1) * kVec - c.lead));
             }
           }
         };

@@ -28,7 +28,6 @@ template <class T, int kMode>
 __global__ void __launch_bounds__(kStreamThreads + 64, 2) distill_stream_kernel(DistillParams p) {
   using R = RowType<T>;
   constexpr int kVec = R::kVec, kWarps = kStreamThreads / 32, kStride = kDisGroup * kStreamThreads;
-  constexpr unsigned kAll = (1u << kVec) - 1u;
   extern __shared__ uint4 stage[];            // the ring; behind it two rows' marks, weights, logits and ids of the list
   __shared__ DistillStreamSmem s;
   const ds41_b200_distill_args &a = p.a;
@@ -49,23 +48,28 @@ __global__ void __launch_bounds__(kStreamThreads + 64, 2) distill_stream_kernel(
     if (kMode == kDistillBoth) return (turn & 1 ? kStreamRing - 1 - g % kStreamRing : g % kStreamRing) * kStride;
     return int((unsigned(turn) * unsigned(groups) + unsigned(g)) % kStreamRing) * kStride;
   };
-  // an id that is not a whole vector's, by its thread: vector v's ids come to, or go from, `at` of the stage
+  // the ids of vector v that are the row's
   auto ids_from = [&](const DistillSlice<T, kStreamThreads> &c, int v) { return max(0, v * kVec - c.lead); };
   auto ids_to = [&](const DistillSlice<T, kStreamThreads> &c, int v) { return min(a.vocab, (v + 1) * kVec - c.lead); };
+  // the copies of a group; what is not the row's is -inf
   auto start_group = [&](const DistillSlice<T, kStreamThreads> &c, int g, int place, bool is) {
     if (is) {
       const int at = g * kStride;
-      const uint32_t to = uint32_t(__cvta_generic_to_shared(stage + place + tid));
+      uint4 *const here = stage + place + tid;
+      const uint32_t to = uint32_t(__cvta_generic_to_shared(here));
 #pragma unroll
-      for (int u = 0; u < kDisGroup; ++u)
+      for (int u = 0; u < kDisGroup; ++u) {
         if (c.whole(at + u * kStreamThreads))
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + u * kStreamThreads * 16), "l"(c.from + at + u * kStreamThreads) : "memory");
+        else
+          here[u * kStreamThreads] = R::nothing();
+      }
       if (c.any_partial()) {
 #pragma unroll 1
         for (int u = 0; u < kDisGroup && at + u * kStreamThreads < c.mine; ++u)
           if (!c.whole(at + u * kStreamThreads)) {
             const int v = tid + at + u * kStreamThreads;
-            copy_ids<T>(reinterpret_cast<T *>(stage + place + u * kStreamThreads + tid) + c.lead - v * kVec, c.x, ids_from(c, v), ids_to(c, v));
+            copy_ids<T>(reinterpret_cast<T *>(here + u * kStreamThreads) + c.lead - v * kVec, c.x, ids_from(c, v), ids_to(c, v));
           }
       }
     }
@@ -134,66 +138,51 @@ __global__ void __launch_bounds__(kStreamThreads + 64, 2) distill_stream_kernel(
       const int *const listed = list_of(turn).ids;
       const float log2e_t = p.log2e_t;
       auto mark = [&](int g) { return unsigned(mark_of[(sizeof(T) == 4 ? g / 2 : g) * kStreamThreads]); };
-      // vector u of group g, as far as its ids are the row's and not listed: the others are -inf
-      auto take = [&](int g, int u, int place, unsigned entry) {
-        const int v = tid + g * kStride + u * kStreamThreads;
-        unsigned some = kAll;
-        if (v * kVec < c.lead) some &= kAll << c.lead;
-        if ((v + 1) * kVec > c.lead + a.vocab) some &= kAll >> ((v + 1) * kVec - c.lead - a.vocab);
-        for (; entry; entry = s.next[turn & 1][entry - 1]) {
-          const int at = listed[entry - 1] + c.lead - v * kVec;
-          if (unsigned(at) < unsigned(kVec)) some &= ~(1u << at);
+      // the thread's vectors of a group that has arrived, listed ids as -inf
+      auto take = [&](int g, int place, uint4 (&q)[kDisGroup]) {
+        uint4 *const here = stage + place + tid;
+#pragma unroll 1
+        for (unsigned entry = mark(g); entry; entry = s.next[turn & 1][entry - 1]) {
+          const int at = listed[entry - 1] + c.lead, v = at / kVec - g * kStride - tid;
+          if (unsigned(v) < unsigned(kStride)) reinterpret_cast<T *>(here + v)[at % kVec] = R::store(-INFINITY);
         }
-        const uint4 q = stage[place + u * kStreamThreads + tid];
-        return some == kAll ? q : R::only(q, some);
+#pragma unroll
+        for (int u = 0; u < kDisGroup; ++u) q[u] = here[u * kStreamThreads];
       };
 
       // ---- maximum and sum of the ids outside the list, forwards
       float high = -FLT_MAX, high_c = -INFINITY, sums[4] = {0.f, 0.f, 0.f, 0.f};   // (relative to high_c)
-      auto raise = [&](float top) {
-        if (top > high) {
-          const float top_c = top * log2e_t;
-          const float down = exp2_approx(near_exponent(top_c) && near_exponent(high_c) ? high_c - top_c : (high - top) * log2e_t);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sums[i] *= down;
-          high = top; high_c = top_c;
-        }
-      };
       float rest_max = -FLT_MAX, rest_sum = 0.f;
       if (kMode != kDistillGrad && !skip) {
 #pragma unroll 1
         for (int g = 0; g < groups; ++g) {
           const int place = place_of(turn, g);
           copies_wait(kStreamRing - 1);
-          const unsigned entry = mark(g);
-          bool fast = entry == 0u && g * kStride + (kDisGroup - 1) * kStreamThreads < c.wholes && !(c.cut && g == 0);
-          if (fast) {
-            uint4 q[kDisGroup];
+          uint4 q[kDisGroup];
+          take(g, place, q);
+          const float top = R::largest(q);
+          if (top > high) {
+            const float top_c = top * log2e_t;
+            const float down = exp2_approx(near_exponent(top_c) && near_exponent(high_c) ? high_c - top_c : (high - top) * log2e_t);
 #pragma unroll
-            for (int u = 0; u < kDisGroup; ++u) q[u] = stage[place + u * kStreamThreads + tid];
-            raise(R::largest(q));
-            fast = near_exponent(high_c);
-            if (fast) {
-#pragma unroll
-              for (int u = 0; u < kDisGroup; ++u) {
-                float y[kVec];
-                R::unpack(q[u], y);
-#pragma unroll
-                for (int k = 0; k < kVec; ++k) sums[k % 4] += exp2_approx(fmaf(y[k], log2e_t, -high_c));
-              }
-            }
+            for (int i = 0; i < 4; ++i) sums[i] *= down;
+            high = top; high_c = top_c;
           }
-          if (!fast) {
-#pragma unroll 1
-            for (int u = 0; u < kDisGroup && g * kStride + u * kStreamThreads < c.mine; ++u) {
-              const uint4 q[1] = {take(g, u, place, entry)};
-              raise(R::largest(q));
-              float y[kVec];
-              R::unpack(q[0], y);
-              const bool is_near = near_exponent(high_c);
-              const float factor = is_near ? 1.f : log2e_t, scaled = is_near ? log2e_t : 1.f, minus = is_near ? -high_c : -high;
+          if (near_exponent(high_c)) {
 #pragma unroll
-              for (int k = 0; k < kVec; ++k) sums[k % 4] += exp2_approx(fmaf(y[k], scaled, minus) * factor);
+            for (int u = 0; u < kDisGroup; ++u) {
+              float y[kVec];
+              R::unpack(q[u], y);
+#pragma unroll
+              for (int k = 0; k < kVec; ++k) sums[k % 4] += exp2_approx(fmaf(y[k], log2e_t, -high_c));
+            }
+          } else {
+#pragma unroll 1
+            for (int u = 0; u < kDisGroup; ++u) {
+              float y[kVec];
+              R::unpack(stage[place + tid + u * kStreamThreads], y);
+#pragma unroll
+              for (int k = 0; k < kVec; ++k) sums[k % 4] += exp2_approx((y[k] - high) * log2e_t);
             }
           }
           const int after = g + kStreamRing;  // (what the ring holds at the end of a first pass stays for the second)
@@ -242,35 +231,39 @@ __global__ void __launch_bounds__(kStreamThreads + 64, 2) distill_stream_kernel(
           for (int i = 0; i < groups; ++i) {
             const int g = kMode == kDistillBoth ? groups - 1 - i : i, place = place_of(turn, g), at = g * kStride;
             copies_wait(kStreamRing - 1);
-            const unsigned entry = mark(g);
-            if (entry == 0u && f.close && by_vectors && at + (kDisGroup - 1) * kStreamThreads < c.wholes && !(c.cut && g == 0)) {
-              uint4 q[kDisGroup];
-#pragma unroll
-              for (int u = 0; u < kDisGroup; ++u) q[u] = stage[place + u * kStreamThreads + tid];
+            uint4 q[kDisGroup];
+            take(g, place, q);
+            if (f.close) {
 #pragma unroll
               for (int u = 0; u < kDisGroup; ++u) {
                 float y[kVec];
                 R::unpack(q[u], y);
 #pragma unroll
                 for (int k = 0; k < kVec; ++k) y[k] = exp2_approx(fmaf(y[k], log2e_t, f.offset));
-                to[at + u * kStreamThreads] = finish_vector(y);
+                q[u] = finish_vector(y);
+                if (by_vectors && c.whole(at + u * kStreamThreads)) to[at + u * kStreamThreads] = q[u];
               }
-            } else {
+            }
+            if (!f.close || !by_vectors || c.any_partial()) {   // by way of the ring, where the vectors are not needed any more
+              uint4 *const here = stage + place + tid;
+              if (f.close) {
+#pragma unroll
+                for (int u = 0; u < kDisGroup; ++u) here[u * kStreamThreads] = q[u];
+              }
 #pragma unroll 1
               for (int u = 0; u < kDisGroup && at + u * kStreamThreads < c.mine; ++u) {
-                float y[kVec];
-                R::unpack(take(g, u, place, entry), y);
+                if (!f.close) {
+                  float y[kVec];
+                  R::unpack(here[u * kStreamThreads], y);
 #pragma unroll
-                for (int k = 0; k < kVec; ++k) y[k] = exp2_approx(fmaf(y[k], f.scaled, f.minus) * f.factor + f.shift);
-                const uint4 q = finish_vector(y);
-                if (by_vectors && c.whole(at + u * kStreamThreads)) {
-                  to[at + u * kStreamThreads] = q;
-                } else {                      // by way of the ring, where the vector is not needed any more
-                  const int v = tid + at + u * kStreamThreads;
-                  uint4 *const here = stage + place + u * kStreamThreads + tid;
-                  *here = q;
-                  copy_ids<T>(grad, reinterpret_cast<const T *>(here) + c.lead - v * kVec, ids_from(c, v), ids_to(c, v));
+                  for (int k = 0; k < kVec; ++k) y[k] = exp2_approx(fmaf(y[k], f.scaled, f.minus) * f.factor + f.shift);
+                  here[u * kStreamThreads] = finish_vector(y);
+                } else if (by_vectors && c.whole(at + u * kStreamThreads)) {
+                  continue;
                 }
+                const int v = tid + at + u * kStreamThreads;
+                if (by_vectors && c.whole(at + u * kStreamThreads)) to[at + u * kStreamThreads] = here[u * kStreamThreads];
+                else copy_ids<T>(grad, reinterpret_cast<const T *>(here + u * kStreamThreads) + c.lead - v * kVec, ids_from(c, v), ids_to(c, v));
               }
             }
             const int after = i + kStreamRing;
