@@ -51,12 +51,19 @@ __global__ void __launch_bounds__(kStreamThreads + 64, 2) distill_stream_kernel(
   // the ids of vector v that are the row's
   auto ids_from = [&](const DistillSlice<T, kStreamThreads> &c, int v) { return max(0, v * kVec - c.lead); };
   auto ids_to = [&](const DistillSlice<T, kStreamThreads> &c, int v) { return min(a.vocab, (v + 1) * kVec - c.lead); };
+  // whether all vectors of a group, every thread's, are whole ones of the row
+  auto inner = [&](const DistillSlice<T, kStreamThreads> &c, int g) { return (g > 0 || c.lead == 0) && (g + 1) * kStride <= (c.lead + a.vocab) / kVec; };
   // the copies of a group; what is not the row's is -inf
   auto start_group = [&](const DistillSlice<T, kStreamThreads> &c, int g, int place, bool is) {
-    if (is) {
-      const int at = g * kStride;
-      uint4 *const here = stage + place + tid;
-      const uint32_t to = uint32_t(__cvta_generic_to_shared(here));
+    const int at = g * kStride;
+    uint4 *const here = stage + place + tid;
+    const uint32_t to = uint32_t(__cvta_generic_to_shared(here));
+    if (is && inner(c, g)) {
+      const uint4 *const from = c.from + at;
+#pragma unroll
+      for (int u = 0; u < kDisGroup; ++u)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + u * kStreamThreads * 16), "l"(from + u * kStreamThreads) : "memory");
+    } else if (is) {
 #pragma unroll
       for (int u = 0; u < kDisGroup; ++u) {
         if (c.whole(at + u * kStreamThreads))
@@ -233,7 +240,9 @@ __global__ void __launch_bounds__(kStreamThreads + 64, 2) distill_stream_kernel(
             copies_wait(kStreamRing - 1);
             uint4 q[kDisGroup];
             take(g, place, q);
+            const bool straight = f.close && by_vectors && inner(c, g);
             if (f.close) {
+              uint4 *const to_group = to + at;
 #pragma unroll
               for (int u = 0; u < kDisGroup; ++u) {
                 float y[kVec];
@@ -241,10 +250,10 @@ __global__ void __launch_bounds__(kStreamThreads + 64, 2) distill_stream_kernel(
 #pragma unroll
                 for (int k = 0; k < kVec; ++k) y[k] = exp2_approx(fmaf(y[k], log2e_t, f.offset));
                 q[u] = finish_vector(y);
-                if (by_vectors && c.whole(at + u * kStreamThreads)) to[at + u * kStreamThreads] = q[u];
+                if (straight) to_group[u * kStreamThreads] = q[u];
               }
             }
-            if (!f.close || !by_vectors || c.any_partial()) {   // by way of the ring, where the vectors are not needed any more
+            if (!straight) {                  // by way of the ring, where the vectors are not needed any more
               uint4 *const here = stage + place + tid;
               if (f.close) {
 #pragma unroll
@@ -258,8 +267,6 @@ __global__ void __launch_bounds__(kStreamThreads + 64, 2) distill_stream_kernel(
 #pragma unroll
                   for (int k = 0; k < kVec; ++k) y[k] = exp2_approx(fmaf(y[k], f.scaled, f.minus) * f.factor + f.shift);
                   here[u * kStreamThreads] = finish_vector(y);
-                } else if (by_vectors && c.whole(at + u * kStreamThreads)) {
-                  continue;
                 }
                 const int v = tid + at + u * kStreamThreads;
                 if (by_vectors && c.whole(at + u * kStreamThreads)) to[at + u * kStreamThreads] = here[u * kStreamThreads];
