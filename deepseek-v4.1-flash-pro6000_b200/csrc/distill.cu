@@ -51,7 +51,8 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
   float *const zs = reinterpret_cast<float *>(ids + 2 * top_room);
   // which ids are in the sum (allowed and not listed): a word holds the bits of the four vectors that a thread takes together
   uint32_t *const bits = reinterpret_cast<uint32_t *>(zs + 2 * top_room);
-  uint32_t *const mask_words = bits + 2 * bits_room;   // of the slice, as they come
+  uint32_t *const mask_words = bits + 2 * bits_room;   // of the slice, as they come, and a zero
+  const int mask_room = p.slice / 32 + 1;
   auto bit_word = [](int v) { return v / (kDisGroup * kCompute) * kCompute + v % kCompute; };
   auto bit_shift = [](int v) { return v / kCompute % kDisGroup * kVec; };
   cudaGridDependencySynchronize();
@@ -98,30 +99,16 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
     uint32_t *const out = bits + (turn & 1) * bits_room;
     if (a.mask) {
       const uint32_t *from = a.mask + size_t(row) * size_t(a.mask_stride) + begin / 32;
-      const int words = min(p.slice / 32, (a.vocab + 31) / 32 - begin / 32);
+      uint32_t *const words = mask_words + (turn & 1) * mask_room;
+      const int count = min(p.slice / 32, (a.vocab + 31) / 32 - begin / 32);
 #pragma unroll 4
-      for (int w = lane; w < words; w += 32)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(uint32_t(__cvta_generic_to_shared(mask_words + w))), "l"(from + w) : "memory");
+      for (int w = lane; w < count; w += 32)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(uint32_t(__cvta_generic_to_shared(words + w))), "l"(from + w) : "memory");
+      if (lane == 0) words[max(count, 0)] = 0u;
       copies_commit();
-      copies_wait(0);
-      __syncwarp();
-#pragma unroll 1
-      for (int w = lane; w < bits_room; w += 32) {
-        uint32_t in = 0u;
-#pragma unroll
-        for (int u = 0; u < kDisGroup; ++u) {
-          const int v = w / kCompute * kDisGroup * kCompute + u * kCompute + w % kCompute;
-          if (v >= c.vecs) continue;
-          const int at = v * kVec - c.lead, low = max(at, 0);          // (the vector's first id; what is in front of the slice is cut off below)
-          uint32_t some = mask_words[low >> 5] >> (low & 31);
-          if ((low & 31) + kVec > 32 && (low >> 5) + 1 < words) some |= mask_words[(low >> 5) + 1] << (32 - (low & 31));
-          in |= ((some << (low - at)) & kAll) << (u * kVec);
-        }
-        out[w] = in;
-      }
-    } else {
-      for (int w = lane; w < bits_room / 4; w += 32) reinterpret_cast<uint4 *>(out)[w] = make_uint4(~0u, ~0u, ~0u, ~0u);
     }
+    for (int w = lane; w < bits_room / 4; w += 32) reinterpret_cast<uint4 *>(out)[w] = make_uint4(~0u, ~0u, ~0u, ~0u);
+    copies_wait(0);
     __syncwarp();
     if (lane == 0) {                          // nothing in front of the slice's first place or behind its last
       out[0] &= ~((1u << c.lead) - 1u);
@@ -216,7 +203,18 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
             if (at + u * kCompute < c.mine) q[u] = here[u * kCompute];
           }
         }
-        const uint32_t in = in_sum[at / kDisGroup] | kNone;
+        uint32_t in = in_sum[at / kDisGroup] | kNone;
+        if (a.mask) {
+          const uint32_t *const words = mask_words + (turn & 1) * mask_room;
+#pragma unroll
+          for (int u = 0; u < kDisGroup; ++u) {
+            const int first = (tid + at + u * kCompute) * kVec - c.lead;   // the vector's first id in the slice
+            uint32_t some = 0u;
+            if (first < 0) some = words[0] << -first;
+            else if (first < len) some = __funnelshift_r(words[first >> 5], words[(first >> 5) + 1], first & 31);
+            in &= ~((~some & kAll) << (u * kVec));
+          }
+        }
         if (in != ~0u) {
 #pragma unroll
           for (int u = 0; u < kDisGroup; ++u) {
@@ -382,7 +380,7 @@ cudaError_t resident_teams(const cudaLaunchConfig_t &cfg, int dev, int team, int
 
 template <int kCompute> size_t distill_smem(int slice, const ds41_b200_distill_args &a, size_t bytes) {
   return size_t(slice) * bytes + 16 + 2 * size_t((a.top + 3) & ~3) * 16 + 2 * size_t(distill_bit_words<kCompute>(slice * int(bytes))) * 4 +
-         (a.mask ? size_t(slice) / 32 * 4 : 0);
+         (a.mask ? 2 * (size_t(slice) / 32 + 1) * 4 : 0);
 }
 
 template <class T, int kMode, int kCompute>
@@ -473,7 +471,7 @@ int distill(const ds41_b200_distill_args *p, cudaStream_t stream) {
     if (!rows_apart_or_same(p->logits, p->logits_stride, p->grad, p->grad_stride, p->rows, p->vocab, bytes))
       return invalid("distill args: grad overlaps logits without being the same rows");
   }
-  DistillParams d{*p, p->grad == p->logits, 0, 1, 0, float(1.4426950408889634 / p->temperature)};
+  DistillParams d{*p, p->grad == p->logits, 0, 1, 0, float(1.4426950408889634 / p->temperature), 1.0 / p->temperature};
   switch (p->dtype) {
     case DS41_B200_F32: return int(launch_distill<float, kMode>(d, stream));
     case DS41_B200_BF16: return int(launch_distill<__nv_bfloat16, kMode>(d, stream));

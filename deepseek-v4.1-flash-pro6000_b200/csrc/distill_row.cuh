@@ -23,6 +23,7 @@ struct DistillParams {
   int slice, team;                            // ids of a CTA (a multiple of 32), CTAs of a row
   int groups;                                 // of a row that is streamed
   float log2e_t;                              // log2(e) / T
+  double inverse_t;                           // 1 / T
 };
 
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -110,7 +111,6 @@ template <class T, int kMode>
 __device__ __forceinline__ void gather_list(const DistillParams &p, int row, DistillRow &r, const DistillList &list_of, int lane) {
   using R = RowType<T>;
   const ds41_b200_distill_args &a = p.a;
-  const double t = a.temperature;
   const int top_room = (a.top + 3) & ~3;
   double *const w_list = list_of.weights;
   int *const id_list = list_of.ids;
@@ -118,31 +118,36 @@ __device__ __forceinline__ void gather_list(const DistillParams &p, int row, Dis
   const T *whole = static_cast<const T *>(a.logits) + size_t(row) * size_t(a.logits_stride);
   const uint32_t *mask = a.mask ? a.mask + size_t(row) * size_t(a.mask_stride) : nullptr;
   const int own = (a.top + 31) / 32;
-  unsigned named = 0u, counts = 0u;         // a bit per entry of the lane
+  // the ids and values, then the logits they name: as many on their way at a time as there are
+#pragma unroll 4
+  for (int k = 0; k < own; ++k) {
+    const int e = lane + 32 * k;
+    if (e >= a.top) break;
+    id_list[e] = load_input(a.teacher_ids + size_t(row) * size_t(a.ids_stride) + e);
+    const size_t at = size_t(row) * size_t(a.values_stride) + e;
+    w_list[e] = a.teacher_dtype == DS41_B200_F64 ? load_input(static_cast<const double *>(a.teacher_values) + at)
+                                                 : double(load_input(static_cast<const float *>(a.teacher_values) + at));
+  }
+#pragma unroll 4
+  for (int k = 0; k < own; ++k) {
+    const int e = lane + 32 * k, id = e < a.top ? id_list[e] : -1;
+    if (id < 0 || id >= a.vocab) continue;
+    const bool is = !mask || ((load_input(mask + (id >> 5)) >> (id & 31)) & 1u);
+    z_list[e] = is ? R::load(whole[id]) : -INFINITY;
+  }
+  unsigned named = 0u, counts = 0u;           // a bit per entry of the lane
   bool bad = false;
   float most = -FLT_MAX, zmax = -FLT_MAX;
 #pragma unroll 1
   for (int k = 0; k < own; ++k) {
-    const int e = lane + 32 * k;
-    int id = -1;
-    double value = 0.0;
-    float z = 0.f;
-    if (e < a.top) {
-      id = load_input(a.teacher_ids + size_t(row) * size_t(a.ids_stride) + e);
-      const size_t at = size_t(row) * size_t(a.values_stride) + e;
-      value = a.teacher_dtype == DS41_B200_F64 ? load_input(static_cast<const double *>(a.teacher_values) + at)
-                                               : double(load_input(static_cast<const float *>(a.teacher_values) + at));
-    }
+    const int e = lane + 32 * k, id = e < a.top ? id_list[e] : -1;
     if (id >= 0 && id < a.vocab) {
+      const float z = z_list[e];
       named |= 1u << k;
-      bad |= !(value < INFINITY);
-      if (!mask || ((load_input(mask + (id >> 5)) >> (id & 31)) & 1u)) {
-        z = R::load(whole[id]);
-        bad |= !(z < INFINITY);
-        if (!(z == -INFINITY)) { counts |= 1u << k; most = fmaxf(most, float(value)); zmax = fmaxf(zmax, z); }
-      }
+      bad |= !(w_list[e] < INFINITY) || !(z < INFINITY);
+      if (!(z == -INFINITY)) { counts |= 1u << k; most = fmaxf(most, float(w_list[e])); zmax = fmaxf(zmax, z); }
     }
-    if (e < top_room) { id_list[e] = (counts >> k) & 1u ? id : -2 - e; w_list[e] = value; z_list[e] = z; }
+    if (e < top_room && !((counts >> k) & 1u)) id_list[e] = -2 - e;
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
@@ -169,14 +174,14 @@ __device__ __forceinline__ void gather_list(const DistillParams &p, int row, Dis
   for (int k = 0; k < own; ++k) {
     const int e = lane + 32 * k;
     if (!((named >> k) & 1u)) continue;
-    const double log_w = a.tail ? w_list[e] : over(w_list[e] - double(most), t), w = exp_of(log_w);
+    const double log_w = a.tail ? w_list[e] : (w_list[e] - double(most)) * p.inverse_t, w = exp_of(log_w);
     list += w;
     const bool is = (counts >> k) & 1u;
     w_list[e] = is ? w : 0.0;
     if (!is) continue;
     kept += w;
     if (!again) {
-      const double gap = over(double(z_list[e]) - double(zmax), t);
+      const double gap = (double(z_list[e]) - double(zmax)) * p.inverse_t;
       if (w > 0.0) entropy += w * (log_w - gap);
       share += exp2_approx((z_list[e] - zmax) * p.log2e_t);
     }
@@ -192,7 +197,7 @@ __device__ __forceinline__ void gather_list(const DistillParams &p, int row, Dis
 #pragma unroll 1
       for (int j = e + 1; j < a.top; ++j)
         if (id_list[j] == id_list[e]) merged[k] += w_list[j];
-      const double gap = over(double(z_list[e]) - double(zmax), t);
+      const double gap = (double(z_list[e]) - double(zmax)) * p.inverse_t;
       if (merged[k] > 0.0) entropy += merged[k] * (log_of(merged[k]) - gap);
       share += exp2_approx((z_list[e] - zmax) * p.log2e_t);
     }
@@ -213,11 +218,11 @@ __device__ __forceinline__ void gather_list(const DistillParams &p, int row, Dis
     share += __shfl_xor_sync(0xffffffffu, share, o);
   }
   bad = __any_sync(0xffffffffu, bad);
+  if (lane < 2) (lane ? r.inverse_rest : r.inverse) = over(1.0, kept + (lane && a.tail ? fmax(0.0, 1.0 - list) : 0.0));
   if (lane == 0) {
     r.reject = bad ? DS41_B200_ROW_NONFINITE : a.tail && list > kDisMost ? DS41_B200_ROW_NOT_NORMALIZED : !(kept > 0.0) ? DS41_B200_ROW_EMPTY : 0;
     r.zmax = zmax; r.share = share; r.kept = kept; r.entropy = entropy;
     r.rest = a.tail ? fmax(0.0, 1.0 - list) : 0.0;
-    r.inverse = over(1.0, kept); r.inverse_rest = over(1.0, kept + r.rest);
     if (kMode == kDistillGrad) r.stats = reinterpret_cast<const float4 *>(a.stats)[row];
   }
   __syncwarp();
@@ -240,7 +245,7 @@ __device__ __forceinline__ void finish_row(const DistillParams &p, int row, cons
   if (!reject) {
     const bool any = rest_sum != 0.f;
     const double zmax = r.zmax, largest = any ? fmax(double(rest_max), zmax) : zmax;
-    const double down = any ? over(double(rest_max) - largest, t) : 0.0, list_down = over(zmax - largest, t);
+    const double down = any ? (double(rest_max) - largest) * p.inverse_t : 0.0, list_down = (zmax - largest) * p.inverse_t;
     const double log_rest = log_of(double(rest_sum));
     const double log_sum = log_of((any ? double(rest_sum) * exp_of(down) : 0.0) + double(r.share) * exp_of(list_down));
     const double inverse = any ? r.inverse_rest : r.inverse, kept = r.kept * inverse, tail = any ? r.rest * inverse : 0.0;
