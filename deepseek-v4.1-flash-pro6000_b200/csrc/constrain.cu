@@ -27,8 +27,9 @@ struct ConstrainParams {
 
 struct Penalty { float repetition, presence, frequency; };
 
-// The sampler's rule, every operation rounded separately.
-__device__ __forceinline__ float penalised(float x, unsigned count, const Penalty &p) {
+// The sampler's rule, every operation rounded separately.  Out of line: it is taken for few ids, from several places, and shall not
+// push the loops out of the instruction cache.
+__device__ __noinline__ float penalised(float x, unsigned count, Penalty p) {
   const float v = x > 0.f ? __fdiv_rn(x, p.repetition) : __fmul_rn(x, p.repetition);
   return __fsub_rn(v, __fadd_rn(p.presence, __fmul_rn(p.frequency, float(count))));
 }
@@ -123,14 +124,16 @@ __global__ void __launch_bounds__(kConThreads, 3) constrain_kernel(ConstrainPara
 #pragma unroll
         for (int k = 0; k < 4; ++k) { count(q[k].x); count(q[k].y); count(q[k].z); count(q[k].w); }
       }
+#pragma unroll 1
       for (; v < vecs4; v += kConThreads) {
         const int4 q = load_input(h4 + v);
         count(q.x); count(q.y); count(q.z); count(q.w);
       }
       i = vecs4 << 2;
     }
-#pragma unroll 4
+#pragma unroll 1
     for (i += tid; i < tokens; i += kConThreads) count(load_input(h + i));
+#pragma unroll 1
     for (int d = tid; d < drafts; d += kConThreads)
       count(load_input(a.draft_ids + size_t(sequence) * size_t(a.rows_per_sequence - 1) + d));
   }
@@ -196,7 +199,7 @@ __global__ void __launch_bounds__(kConThreads, 3) constrain_kernel(ConstrainPara
     }
     if (!R::all_finite(finite)) poison = __int_as_float(0x7fffffff);
   } else {                                         // rows whose vectors do not line up with the output's: id by id
-#pragma unroll 4
+#pragma unroll 2
     for (int i = tid; i < len; i += kConThreads) copy(i);
   }
   if (!(pen.repetition > 0.f) || !finite_bits(pen.repetition) || !finite_bits(pen.presence) || !finite_bits(pen.frequency))
@@ -204,12 +207,14 @@ __global__ void __launch_bounds__(kConThreads, 3) constrain_kernel(ConstrainPara
   // (counts and copies are done.)  Does the mask allow any id?  The other slices are looked at only by a CTA whose own allows none
   if (!__syncthreads_or(int(any)) && mask) {
     const int words = (a.vocab + 31) / 32;
+#pragma unroll 1
     for (int w = tid; w < words; w += kConThreads)
       any |= load_input(mask + w) & (w == words - 1 && (a.vocab & 31) ? (1u << (a.vocab & 31)) - 1u : ~0u);
     if (!__syncthreads_or(int(any)) && !reject) reject = DS41_B200_ROW_EMPTY;
   }
   if (reject) {                                    // the same in every CTA of the team
     const T nan = R::store(__int_as_float(0x7fffffff));
+#pragma unroll 1
     for (int i = tid; i < len; i += kConThreads) out[i] = nan;
     if (rank == 0 && tid == 0 && a.status) a.status[row] = reject;
     return;
@@ -235,15 +240,17 @@ __global__ void __launch_bounds__(kConThreads, 3) constrain_kernel(ConstrainPara
     }
     __syncthreads();                               // (every entry has its count)
     const bool twice = listed_twice != 0;
-#pragma unroll
+#pragma unroll 1
     for (int k = 0; k < kConOwn; ++k)
       if (listed[k] >= 0) {
         atomicAnd(&counts[listed[k] >> 1], (unsigned(listed[k]) & 1u) ? 0xffffu : 0xffff0000u);   // settled here
         if (twice) {                               // the id's first entry adds the later ones, which drop out
           const int id = begin + listed[k], e = tid + k * kConThreads;
           bool is_first = true;
+#pragma unroll 1
           for (int o = 0; o < e && is_first; ++o) is_first = load_input(bias_ids + o) != id;
           if (!is_first) continue;
+#pragma unroll 1
           for (int o = e + 1; o < a.biases; ++o)
             if (load_input(bias_ids + o) == id) bias[k] = __fadd_rn(bias[k], load_input(bias_values + o));
         }
@@ -263,6 +270,7 @@ __global__ void __launch_bounds__(kConThreads, 3) constrain_kernel(ConstrainPara
       const uint32_t some = __vminu2(q.x, 0x10001u) | __vminu2(q.y, 0x10001u) << 1 | __vminu2(q.z, 0x10001u) << 2 | __vminu2(q.w, 0x10001u) << 3;
       bits |= some << (4 * k);
     }
+#pragma unroll 1
     for (; bits; bits &= bits - 1u) {
       const int bit = __ffs(bits) - 1, local = 8 * (tid + ((bit >> 2) & 3) * kConThreads) + 2 * (bit & 3) + (bit >> 4);
       if (!allowed(local)) continue;
