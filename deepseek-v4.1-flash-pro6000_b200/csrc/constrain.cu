@@ -296,11 +296,14 @@ __global__ void __launch_bounds__(kConThreads, 3) constrain_kernel(ConstrainPara
   }
 }
 
-// Rows up to which the CTAs of a row form a cluster and settle its status among themselves.  Beyond, each adds its flags to the status
-// words, cleared by a node in front of the kernel: a cluster starts when all its CTAs have a place, and leaves together.
-constexpr int kConTeamRows = 16;
+// CTAs up to which those of a row form a cluster and settle its status among themselves: as many as run at a time.  Beyond, each adds its
+// flags to the status words, cleared by a node in front of the kernel, since a cluster starts when all its CTAs have a place, and
+// leaves together.  Cluster / cleared words, us, fp32 rows with 2048 tokens: 129280 ids 1 row 6.0 / 8.3, 32 rows 11.7 / 14.3, 48 rows 14.2 / 16.5,
+// 96 rows 27.2 / 26.7, 256 rows 68 / 55; 32000 ids 96 rows 11.6 / 14.4, 256 rows 26.9 / 26.5.
+constexpr int kConTeamCtas = 3 * 148;
 
-// CTAs per row: as few as the counters allow, and for batches that leave SMs idle up to eight, of at least 2048 ids each.
+// CTAs per row: as few as the counters allow, and for batches that leave SMs idle up to eight, of at least 2048 ids each.  Two CTAs / up to
+// eight for 32000 ids, us: 1 row 7.4 / 4.9, 24 rows 10.3 / 5.8, 32 rows 10.3 / 6.6.
 int constrain_team(int rows, int vocab) {
   int n = (vocab + kConSlice - 1) / kConSlice;
   while (n < 8 && 2LL * rows * n <= 148 && vocab > n * 2048) ++n;
@@ -320,7 +323,7 @@ cudaError_t launch_constrain(const ds41_b200_constrain_args &a, int rows, cudaSt
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = unsigned(team); attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr; cfg.numAttrs = 2;
-  if (rows <= kConTeamRows || !a.status) return cudaLaunchKernelEx(&cfg, constrain_kernel<T, true>, p);
+  if ((long long)rows * team <= kConTeamCtas || !a.status) return cudaLaunchKernelEx(&cfg, constrain_kernel<T, true>, p);
   cfg.numAttrs = 1;
   const cudaError_t e = cudaMemsetAsync(a.status, 0, size_t(rows) * sizeof(int32_t), stream);
   if (e != cudaSuccess) return e;

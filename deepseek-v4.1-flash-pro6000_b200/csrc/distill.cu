@@ -440,7 +440,9 @@ cudaError_t launch_distill(DistillParams &d, cudaStream_t stream) {
   while (d.team < 8 && (slice(d.team) > kLarge || distill_smem<256>(slice(d.team), d.a, sizeof(T)) > 74 * 1024)) ++d.team;
   while (d.team < 8 && 2LL * d.a.rows * d.team <= 148 && vocab > d.team * 4096) ++d.team;
   d.slice = slice(d.team);
-  return d.slice <= kSmall ? launch_distill<T, kMode, 64>(d, stream) : launch_distill<T, kMode, 256>(d, stream);
+  // Few compute threads a CTA where there are more rows than the wide ones take at a time.  64 / 256 threads, us, bf16 loss and gradient, one
+  // CTA per row: 4000 ids 128 rows 9.6 / 8.7, 600 rows 12.1 / 17.6, 5000 rows 51 / 91; 1031 ids 600 rows 10.6 / 17.3
+  return d.slice <= kSmall && (long long)d.a.rows * d.team > 3 * 148 ? launch_distill<T, kMode, 64>(d, stream) : launch_distill<T, kMode, 256>(d, stream);
 }
 
 template <int kMode>
