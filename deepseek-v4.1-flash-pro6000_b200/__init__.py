@@ -176,16 +176,18 @@ _ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # DS41_B2
 
 def _rows(t, dtypes, name, device, shape):
     """The row stride of a 2-D tensor of that shape (None: any extent) with unit inner stride on `device`."""
-    if not t.is_cuda or t.device != device or t.dtype not in dtypes or t.dim() != 2 or \
-            any(n is not None and n != m for n, m in zip(shape, t.shape)) or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name} must be a tensor of {' or '.join(map(str, dtypes))} on {device} of {shape} rows and columns, "
-                         f"columns next to each other")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if t.dim() == 2 and t.device == device and t.dtype in dtypes:
+        rows, columns = t.shape
+        stride, inner = t.stride()
+        if rows == shape[0] and (shape[1] is None or columns == shape[1]) and (inner == 1 or columns <= 1):
+            return stride if rows > 1 else columns
+    raise ValueError(f"{name} must be a tensor of {' or '.join(map(str, dtypes))} on {device} of {tuple(shape)} rows and columns, "
+                     f"columns next to each other")
 
 
 def _flat(t, dtype, name, device, count):
     """`t` itself, checked: contiguous, on `device`, `count` elements."""
-    if not t.is_cuda or t.device != device or t.dtype != dtype or t.numel() != count or not t.is_contiguous():
+    if t.device != device or t.dtype != dtype or t.numel() != count or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous tensor of {count} {dtype} on {device}")
     return t
 
@@ -509,34 +511,23 @@ def score_logits(logits, top_n=0):
     return lse, top1, ids, lp, status
 
 
-def _distill_args(logits, teacher_ids, teacher_values, temperature, tail, mask, row_scale):
-    """What the three calls share, checked."""
+def _distill(name, logits, teacher_ids, teacher_values, temperature, tail, mask, row_scale, loss=None, stats=None, out=None, status=None):
+    """One of the three calls on checked tensors."""
     if logits.dim() != 2 or not logits.is_cuda or logits.dtype not in _ROW_TYPES:
         raise ValueError("logits must be a CUDA fp32, bf16 or fp16 [rows, vocab] tensor")
-    rows, vocab = logits.shape
-    dev = logits.device
-    a = DistillArgs()
-    a.struct_bytes = C.sizeof(DistillArgs)
-    a.rows, a.vocab, a.dtype, a.tail = rows, vocab, _ROW_TYPES[logits.dtype], 1 if tail else 0
-    a.logits, a.logits_stride = logits.data_ptr(), _rows(logits, (logits.dtype,), "logits", dev, (rows, vocab))
-    a.ids_stride = _rows(teacher_ids, (torch.int32,), "teacher_ids", dev, (rows, None))
-    a.top = teacher_ids.shape[1]
-    a.values_stride = _rows(teacher_values, (torch.float32, torch.float64), "teacher_values", dev, (rows, a.top))
-    a.teacher_ids, a.teacher_values = teacher_ids.data_ptr(), teacher_values.data_ptr()
-    a.teacher_dtype = 3 if teacher_values.dtype == torch.float64 else 0
-    a.temperature = temperature
-    if mask is not None:
-        a.mask, a.mask_stride = mask.data_ptr(), _rows(mask, (torch.int32,), "mask", dev, (rows, None))
-    if row_scale is not None:
-        a.row_scale = _flat(row_scale, torch.float32, "row_scale", dev, rows).data_ptr()
-    return a
-
-
-def _distill_grad_buffer(a, logits, out):
-    if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    a.grad, a.grad_stride = out.data_ptr(), _rows(out, (logits.dtype,), "out", logits.device, logits.shape)
-    return out
+    shape, dev, dtype = logits.shape, logits.device, logits.dtype
+    rows, vocab = shape
+    stride = _rows(logits, (dtype,), "logits", dev, shape)
+    ids_stride = _rows(teacher_ids, (torch.int32,), "teacher_ids", dev, (rows, None))
+    top = teacher_ids.shape[1]
+    values_stride = _rows(teacher_values, (torch.float32, torch.float64), "teacher_values", dev, (rows, top))
+    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+    a = DistillArgs(C.sizeof(DistillArgs), rows, vocab, _ROW_TYPES[dtype], 3 if teacher_values.dtype == torch.float64 else 0, top,
+                    1 if tail else 0, 0, logits.data_ptr(), stride, teacher_ids.data_ptr(), ids_stride, teacher_values.data_ptr(),
+                    values_stride, temperature, ptr(mask), _rows(mask, (torch.int32,), "mask", dev, (rows, None)) if mask is not None else 0,
+                    _flat(row_scale, torch.float32, "row_scale", dev, rows).data_ptr() if row_scale is not None else None, ptr(loss),
+                    ptr(stats), ptr(out), _rows(out, (dtype,), "out", dev, shape) if out is not None else 0, ptr(status))
+    _launch(dev, name, getattr(lib(), name), C.byref(a))
 
 
 def distill_loss(logits, teacher_ids, teacher_values, temperature=1.0, tail=False, mask=None):
@@ -546,13 +537,11 @@ def distill_loss(logits, teacher_ids, teacher_values, temperature=1.0, tail=Fals
     list; tail=True (temperature 1): the values are log-probabilities, and what they leave belongs to the ids outside the list.
     mask int32 [rows, >= ceil(vocab / 32)]: allowed-token bits, as in sample_logits; a logit of -inf is not allowed either.
     Returns (loss fp32 [rows], stats fp32 [rows, 4] for distill_grad, status int32 [rows]); see ds41_b200.h for the formulas."""
-    a = _distill_args(logits, teacher_ids, teacher_values, temperature, tail, mask, None)
-    dev = logits.device
-    loss = torch.empty(a.rows, dtype=torch.float32, device=dev)
-    stats = torch.empty((a.rows, 4), dtype=torch.float32, device=dev)
-    status = torch.empty(a.rows, dtype=torch.int32, device=dev)
-    a.loss, a.stats, a.status = loss.data_ptr(), stats.data_ptr(), status.data_ptr()
-    _launch(dev, "ds41_b200_distill_loss", lib().ds41_b200_distill_loss, C.byref(a))
+    rows, dev = logits.shape[0], logits.device
+    loss = torch.empty(rows, dtype=torch.float32, device=dev)
+    stats = torch.empty((rows, 4), dtype=torch.float32, device=dev)
+    status = torch.empty(rows, dtype=torch.int32, device=dev)
+    _distill("ds41_b200_distill_loss", logits, teacher_ids, teacher_values, temperature, tail, mask, None, loss, stats, None, status)
     return loss, stats, status
 
 
@@ -560,12 +549,12 @@ def distill_grad(logits, teacher_ids, teacher_values, stats, row_scale=None, tem
     """The gradient of row_scale[r] * loss[r] by logits (the upstream gradient of each row's loss; None = 1; rows with 0 are not
     read) from distill_loss's stats and the same other arguments.  out: None allocates; logits itself works in place.
     Returns the gradient in the logits' type."""
-    a = _distill_args(logits, teacher_ids, teacher_values, temperature, tail, mask, row_scale)
     if stats.dim() != 2 or stats.shape[1] != 4:
         raise ValueError("stats must be [rows, 4]")
-    a.stats = _flat(stats, torch.float32, "stats", logits.device, 4 * a.rows).data_ptr()
-    out = _distill_grad_buffer(a, logits, out)
-    _launch(logits.device, "ds41_b200_distill_grad", lib().ds41_b200_distill_grad, C.byref(a))
+    _flat(stats, torch.float32, "stats", logits.device, 4 * logits.shape[0])
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    _distill("ds41_b200_distill_grad", logits, teacher_ids, teacher_values, temperature, tail, mask, row_scale, None, stats, out)
     return out
 
 
@@ -573,13 +562,12 @@ def distill_loss_grad(logits, teacher_ids, teacher_values, row_scale=None, tempe
     """Loss and gradient in one call that reads the logits once: distill_loss and distill_grad with row_scale known beforehand
     (rows with 0 are not read: loss 0, gradient 0).  out: None allocates; logits itself works in place.
     Returns (loss fp32 [rows], gradient in the logits' type, status int32 [rows])."""
-    a = _distill_args(logits, teacher_ids, teacher_values, temperature, tail, mask, row_scale)
-    dev = logits.device
-    loss = torch.empty(a.rows, dtype=torch.float32, device=dev)
-    status = torch.empty(a.rows, dtype=torch.int32, device=dev)
-    a.loss, a.status = loss.data_ptr(), status.data_ptr()
-    out = _distill_grad_buffer(a, logits, out)
-    _launch(dev, "ds41_b200_distill_loss_grad", lib().ds41_b200_distill_loss_grad, C.byref(a))
+    rows, dev = logits.shape[0], logits.device
+    loss = torch.empty(rows, dtype=torch.float32, device=dev)
+    status = torch.empty(rows, dtype=torch.int32, device=dev)
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    _distill("ds41_b200_distill_loss_grad", logits, teacher_ids, teacher_values, temperature, tail, mask, row_scale, loss, None, out, status)
     return loss, out, status
 
 
