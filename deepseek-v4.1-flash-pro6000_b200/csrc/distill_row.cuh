@@ -137,7 +137,8 @@ __device__ __forceinline__ void gather_list(const DistillParams &p, int row, Dis
   }
   unsigned named = 0u, counts = 0u;           // a bit per entry of the lane
   bool bad = false;
-  float most = -FLT_MAX, zmax = -FLT_MAX;
+  double most = -DBL_MAX;
+  float zmax = -FLT_MAX;
 #pragma unroll 1
   for (int k = 0; k < own; ++k) {
     const int e = lane + 32 * k, id = e < a.top ? id_list[e] : -1;
@@ -145,13 +146,13 @@ __device__ __forceinline__ void gather_list(const DistillParams &p, int row, Dis
       const float z = z_list[e];
       named |= 1u << k;
       bad |= !(w_list[e] < INFINITY) || !(z < INFINITY);
-      if (!(z == -INFINITY)) { counts |= 1u << k; most = fmaxf(most, float(w_list[e])); zmax = fmaxf(zmax, z); }
+      if (!(z == -INFINITY)) { counts |= 1u << k; most = fmax(most, w_list[e]); zmax = fmaxf(zmax, z); }
     }
     if (e < top_room && !((counts >> k) & 1u)) id_list[e] = -2 - e;
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    most = fmax(most, __shfl_xor_sync(0xffffffffu, most, o));
     zmax = fmaxf(zmax, __shfl_xor_sync(0xffffffffu, zmax, o));
   }
   __syncwarp();
@@ -174,7 +175,7 @@ __device__ __forceinline__ void gather_list(const DistillParams &p, int row, Dis
   for (int k = 0; k < own; ++k) {
     const int e = lane + 32 * k;
     if (!((named >> k) & 1u)) continue;
-    const double log_w = a.tail ? w_list[e] : (w_list[e] - double(most)) * p.inverse_t, w = exp_of(log_w);
+    const double log_w = a.tail ? w_list[e] : (w_list[e] - most) * p.inverse_t, w = exp_of(log_w);
     list += w;
     const bool is = (counts >> k) & 1u;
     w_list[e] = is ? w : 0.0;
@@ -312,8 +313,8 @@ __device__ __forceinline__ DistillFactors gradient_factors(const DistillParams &
   }
   f.rest_max = rest_max; f.rest_sum = rest_sum;
   const float tail = any ? float(r.rest * r.inverse_rest) : 0.f, coef = any ? r.scale * float(p.a.temperature) * (q_rest - tail) / rest_sum : 0.f;
-  // 16-bit types: the factor's size goes into the exponent, its sign into the words (exponents below 256 are off by 2^-17, a power
-  // by 2^-17, which is little beside the rounding to 16 bits)
+  // 16-bit types: the factor's size goes into the exponent, its sign into the words (exponents below 512 are off by 2^-16, a power
+  // by as much, which is little beside the rounding to 16 bits)
   const float rest_c = rest_max * log2e_t, over_c = excess(rest_max, log2e_t, rest_c);
   f.close = kBytes == 4 ? near_exponent(rest_c) : fabsf(rest_c) < 256.f;
   const float shift = kBytes == 4 ? 0.f : log2f(fabsf(coef));

@@ -6,6 +6,8 @@ and runs too long to be replayed pass after pass).
     python deepseek-v4.1-flash-pro6000_b200/profile_cases.py headbf16 [--rows 6]        (the reference's BF16 plugin shape)
     python deepseek-v4.1-flash-pro6000_b200/profile_cases.py sampler [--rows 64] [--dist flat|peaked] [--stream]
     python deepseek-v4.1-flash-pro6000_b200/profile_cases.py verify  [--seqs 8] [--drafts 2]
+    python deepseek-v4.1-flash-pro6000_b200/profile_cases.py constrain [--rows 256] [--history 32768] [--masked]
+    python deepseek-v4.1-flash-pro6000_b200/profile_cases.py distill [--rows 1024] [--masked]      (bf16, loss and gradient)
 
 Each case launches its kernel `--repeat` times (default 3) after one warm-up call and checks the status words.  Inputs
 are larger than the 126 MB L2 only where the kernel's DRAM figures are the point (sampler: rows * 517 KB); the head case
@@ -22,7 +24,7 @@ VOCAB = 129280
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("case", choices=["head", "headbf16", "sampler", "verify"])
+    ap.add_argument("case", choices=["head", "headbf16", "sampler", "verify", "constrain", "distill"])
     ap.add_argument("--rows", type=int, default=None)
     ap.add_argument("--vocab", type=int, default=16384)
     ap.add_argument("--hidden", type=int, default=4096)
@@ -30,6 +32,8 @@ def main():
     ap.add_argument("--stream", action="store_true", help="sampler: give it scratch, i.e. allow the streaming path")
     ap.add_argument("--seqs", type=int, default=8)
     ap.add_argument("--drafts", type=int, default=2)
+    ap.add_argument("--history", type=int, default=4096)
+    ap.add_argument("--masked", action="store_true", help="constrain, distill: a random bitmask that allows an eighth of the ids")
     ap.add_argument("--repeat", type=int, default=3)
     args = ap.parse_args()
     import torch
@@ -74,6 +78,28 @@ def main():
             tok, st = pkg.sample_logits(x, 0.6, 0.95, seeds, steps, scratch="auto" if args.stream else None)
         torch.cuda.synchronize()
         assert (st >= 0).all()
+    elif args.case in ("constrain", "distill"):
+        rows = args.rows or (256 if args.case == "constrain" else 1024)
+        mask = None
+        if args.masked:   # three random words: a bit of their conjunction is set in one of eight
+            words = [torch.randint(-2 ** 31, 2 ** 31 - 1, (rows, VOCAB // 32), device=dev, dtype=torch.int32, generator=g) for _ in range(3)]
+            mask = words[0] & words[1] & words[2]
+        x = 3.0 * torch.randn(rows, VOCAB, device=dev, generator=g)
+        if args.case == "constrain":
+            history = torch.randint(0, VOCAB, (rows, args.history), device=dev, dtype=torch.int32, generator=g)
+            out = torch.empty_like(x)
+            for _ in range(1 + args.repeat):
+                _, st = pkg.constrain_logits(x, history=history, repetition=1.1, presence=0.3, frequency=0.2, mask=mask, out=out)
+        else:
+            _, _, ids, logprobs, _ = pkg.score_logits(x, 32)
+            z = (x + torch.randn(rows, VOCAB, device=dev, generator=g)).to(torch.bfloat16)
+            out = torch.empty_like(z)
+            del x
+            torch.cuda.empty_cache()
+            for _ in range(1 + args.repeat):
+                _, _, st = pkg.distill_loss_grad(z, ids, logprobs, tail=True, mask=mask, out=out)
+        torch.cuda.synchronize()
+        assert (st <= 0).all() and (st == 0).any()
     else:
         seqs, d = args.seqs, args.drafts
         target = 3.0 * torch.randn(seqs * (d + 1), VOCAB, device=dev, generator=g)
