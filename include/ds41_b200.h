@@ -390,7 +390,8 @@ typedef struct ds41_b200_constrain_args {
   int32_t biases;              /* entries of a sequence's bias list, 0..DS41_B200_CONSTRAIN_MAX_BIASES */
   const void *logits;          /* [rows, logits_stride] */
   int64_t logits_stride;       /* elements: >= vocab, or 0 to give every row the same logits */
-  void *out;                   /* [rows, out_stride]; may be logits with the same stride (in place), no other overlap */
+  void *out;                   /* [rows, out_stride]; may be logits with the same stride (in place), no other overlap.  Rows that lie
+                                  otherwise to 16 bytes than the logits' are written id by id, which is slower */
   int64_t out_stride;
   float repetition, presence, frequency; /* for every sequence, where penalties is NULL; 1,0,0 = off */
   float fill;
@@ -452,7 +453,7 @@ typedef struct ds41_b200_distill_args {
   const float *row_scale;      /* [rows] or NULL; of the gradient's calls */
   float *loss;                 /* [rows] out */
   float *stats;                /* [rows, 4] out; in for _grad; 16-byte aligned */
-  void *grad;                  /* [rows, grad_stride] out */
+  void *grad;                  /* [rows, grad_stride] out; rows that lie otherwise to 16 bytes than the logits' take longer */
   int64_t grad_stride;
   int32_t *status;             /* [rows] out */
 } ds41_b200_distill_args;

@@ -63,7 +63,8 @@ def test_rows_of_every_size_type_and_alignment(pkg, dtype, vocab, lead, gap, top
 
 @pytest.mark.parametrize("rows,vocab,top,tail,temperature,share", [
     (1, 129280, 20, True, 1.0, None), (2, 129280, 1, False, 0.5, 0.02), (60, 40001, 64, True, 1.0, 0.3), (300, 5003, 17, False, 4.0, None),
-    (150, 65537, 33, True, 1.0, None), (1000, 257, 256, False, 1.5, 0.9), (37, 100000, 8, True, 1.0, 0.0005)])
+    (150, 65537, 33, True, 1.0, None), (147, 40001, 5, True, 1.0, None), (148, 40001, 5, False, 1.3, None), (148, 36857, 9, True, 1.0, None),
+    (148, 36865, 255, True, 1.0, None), (148, 36865, 256, False, 1.0, None), (444, 1031, 7, True, 1.0, 0.5), (445, 1031, 7, True, 1.0, 0.5), (1000, 257, 256, False, 1.5, 0.9), (37, 100000, 8, True, 1.0, 0.0005)])
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_batches(pkg, rows, vocab, top, tail, temperature, share, dtype):
     check(pkg, case(rows + vocab, rows, vocab, TYPES[dtype], top, tail, share), TYPES[dtype], temperature, tail)
