@@ -185,6 +185,15 @@ def _rows(t, dtypes, name, device, shape):
                      f"columns next to each other")
 
 
+def _mask(t, device, rows, vocab):
+    """Address and row stride of a bitmask.  Its columns are counted here: a view cut out of wider rows has their stride, and one without
+    columns has no address, so the library could tell neither.  (The same kind of error as the library's for a stride that is too short.)"""
+    stride, words = _rows(t, (torch.int32,), "mask", device, (rows, None)), (vocab + 31) // 32
+    if t.shape[1] < words:
+        raise RuntimeError(f"mask has {t.shape[1]} words a row, {vocab} ids take {words} (mask stride or width shorter than the vocabulary)")
+    return t.data_ptr(), stride
+
+
 def _flat(t, dtype, name, device, count):
     """`t` itself, checked: contiguous, on `device`, `count` elements."""
     if t.device != device or t.dtype != dtype or t.numel() != count or not t.is_contiguous():
@@ -308,7 +317,7 @@ def constrain_logits(logits, history=None, history_len=None, repetition=1.0, pre
         raise ValueError("history_len without history")
     if (bias_ids is None) != (bias_values is None):
         raise ValueError("bias_ids and bias_values come together")
-    history_stride = biases = mask_stride = 0
+    history_stride = biases = 0
     if history is not None:
         history_stride = _rows(_flat(history, torch.int32, "history", dev, history.numel()), (torch.int32,), "history", dev,
                                (sequences, None))
@@ -322,8 +331,7 @@ def constrain_logits(logits, history=None, history_len=None, repetition=1.0, pre
         biases = bias_ids.shape[-1]
         _flat(bias_ids, torch.int32, "bias_ids", dev, sequences * biases)
         _flat(bias_values, torch.float32, "bias_values", dev, sequences * biases)
-    if mask is not None:
-        mask_stride = _rows(mask, (torch.int32,), "mask", dev, (rows, None))
+    mask_ptr, mask_stride = _mask(mask, dev, rows, vocab) if mask is not None else (None, 0)
     lowest = torch.finfo(logits.dtype).min
     if fill is None:
         fill = lowest
@@ -332,7 +340,7 @@ def constrain_logits(logits, history=None, history_len=None, repetition=1.0, pre
     ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
     a = ConstrainArgs(C.sizeof(ConstrainArgs), sequences, rows_per_sequence, vocab, _ROW_TYPES[logits.dtype], biases, logits.data_ptr(),
                       logits_stride, out.data_ptr(), out_stride, repetition, presence, frequency, fill, ptr(penalties), ptr(history), history_stride,
-                      ptr(history_len), ptr(draft_ids), ptr(bias_ids), ptr(bias_values), ptr(mask), mask_stride, status.data_ptr())
+                      ptr(history_len), ptr(draft_ids), ptr(bias_ids), ptr(bias_values), mask_ptr, mask_stride, status.data_ptr())
     _launch(dev, "ds41_b200_constrain_logits", lib().ds41_b200_constrain_logits, C.byref(a))
     return out, status
 
@@ -521,10 +529,11 @@ def _distill(name, logits, teacher_ids, teacher_values, temperature, tail, mask,
     ids_stride = _rows(teacher_ids, (torch.int32,), "teacher_ids", dev, (rows, None))
     top = teacher_ids.shape[1]
     values_stride = _rows(teacher_values, (torch.float32, torch.float64), "teacher_values", dev, (rows, top))
+    mask_ptr, mask_stride = _mask(mask, dev, rows, vocab) if mask is not None else (None, 0)
     ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
     a = DistillArgs(C.sizeof(DistillArgs), rows, vocab, _ROW_TYPES[dtype], 3 if teacher_values.dtype == torch.float64 else 0, top,
                     1 if tail else 0, 0, logits.data_ptr(), stride, teacher_ids.data_ptr(), ids_stride, teacher_values.data_ptr(),
-                    values_stride, temperature, ptr(mask), _rows(mask, (torch.int32,), "mask", dev, (rows, None)) if mask is not None else 0,
+                    values_stride, temperature, mask_ptr, mask_stride,
                     _flat(row_scale, torch.float32, "row_scale", dev, rows).data_ptr() if row_scale is not None else None, ptr(loss),
                     ptr(stats), ptr(out), _rows(out, (dtype,), "out", dev, shape) if out is not None else 0, ptr(status))
     _launch(dev, name, getattr(lib(), name), C.byref(a))
