@@ -299,7 +299,7 @@ __device__ __forceinline__ DistillFactors gradient_factors(const DistillParams &
   if (kMode == kDistillGrad) {
     f.largest = r.stats.x; f.inverse_sum = exp2_approx(-r.stats.y * 1.44269504f);
     any = r.stats.w > -INFINITY;
-    rest_max = any ? r.stats.z : 0.f;
+    rest_max = r.stats.z;
     rest_sum = any ? exp2_approx(r.stats.w * 1.44269504f) : 0.f;
     q_rest = any ? rest_sum * exp2_approx((rest_max - f.largest) * log2e_t) * f.inverse_sum : 0.f;
     if (!f.reject && !(r.stats.x == r.stats.x)) f.reject = DS41_B200_ROW_NONFINITE;
@@ -311,6 +311,8 @@ __device__ __forceinline__ DistillFactors gradient_factors(const DistillParams &
     q_rest = part * f.inverse_sum;
     if (!f.reject && !(rest_sum < INFINITY)) f.reject = DS41_B200_ROW_NONFINITE;
   }
+  // (no ids outside the list: a maximum of theirs that is none would make the power's correction below infinite, and 0 times it NaN)
+  if (!any) rest_max = 0.f;
   f.rest_max = rest_max; f.rest_sum = rest_sum;
   const float tail = any ? float(r.rest * r.inverse_rest) : 0.f, coef = any ? r.scale * float(p.a.temperature) * (q_rest - tail) / rest_sum : 0.f;
   // 16-bit types: the factor's size goes into the exponent, its sign into the words (exponents below 512 are off by 2^-16, a power
