@@ -233,8 +233,8 @@ __global__ void __launch_bounds__(kCompute + 64, kCompute == 256 ? 3 : 8) distil
         take(at, kMode == kDistillBoth, q);
         const float top = R::largest(q);
         if (top > high) {
-          const float top_c = top * log2e_t;
-          const float down = exp2_approx(near_exponent(top_c) && near_exponent(high_c) ? high_c - top_c : (high - top) * log2e_t);
+          const float top_c = rounded_product(top, log2e_t);
+          const float down = rise(high, high_c, top, top_c, log2e_t);
 #pragma unroll
           for (int i = 0; i < 4; ++i) sums[i] *= down;
           high = top; high_c = top_c;

@@ -47,12 +47,21 @@ __device__ __forceinline__ float exp2_approx(float x) {   // 2 ulp; 0 for -inf a
   return y;
 }
 
-// An exponent of two below which, and above whose negative, a product of logit and log2(e) / T is taken as it is: the power of
-// x c - r with r = m c rounded is one fused multiply-add, its argument as exact as that of (x - m) c, if the rounding of r is made good for
-// once a row.  Beyond (rows of a type's lowest values) it is (x - m) c.
-constexpr float kDisNear = 1e37f;
+// The power of (x - m) c, with c = log2(e) / T, as that of x c - r with r = m c rounded: one fused multiply-add, its argument as exact, if
+// the rounding of r is made good for once a row.  That rounding is up to 2^-24 |r|, so the shortcut is for |r| below 2^24, where its power lies
+// between 0.7 and 1.42; at 2^31 it would be infinite or 0.  Beyond (logits of -1e8 and less in a row's masked places, a type's lowest values)
+// the power is that of (x - m) c.  (The rounding is asked for by name: what takes r must not get the product that it was rounded from.)
+constexpr float kDisNear = 16777216.f;
 __device__ __forceinline__ bool near_exponent(float r) { return fabsf(r) < kDisNear; }
+__device__ __forceinline__ float rounded_product(float m, float c) { return __fmul_rn(m, c); }
 __device__ __forceinline__ float excess(float m, float c, float r) { return near_exponent(r) ? fmaf(m, c, -r) : 0.f; }
+// What a sum of such powers relative to m is multiplied by where the maximum rises to `top`: it stands relative to r where that is near, and
+// to the product itself where it is not, whichever side either is on.  (The maximum before the first has r = -inf.)
+__device__ __forceinline__ float rise(float m, float r, float top, float top_r, float c) {
+  const float down = near_exponent(top_r) ? (near_exponent(r) ? __fsub_rn(r, top_r) : fmaf(m, c, -top_r))
+                                          : (near_exponent(r) ? -fmaf(top, c, -r) : (m - top) * c);
+  return exp2_approx(down);
+}
 
 // Out of line, once each: what runs a few times a row shall not push the loops out of the instruction cache.
 __device__ __noinline__ double exp_of(double x) { return exp(x); }
@@ -317,11 +326,11 @@ __device__ __forceinline__ DistillFactors gradient_factors(const DistillParams &
   const float tail = any ? float(r.rest * r.inverse_rest) : 0.f, coef = any ? r.scale * float(p.a.temperature) * (q_rest - tail) / rest_sum : 0.f;
   // 16-bit types: the factor's size goes into the exponent, its sign into the words (exponents below 512 are off by 2^-16, a power
   // by as much, which is little beside the rounding to 16 bits)
-  const float rest_c = rest_max * log2e_t, over_c = excess(rest_max, log2e_t, rest_c);
+  const float rest_c = rounded_product(rest_max, log2e_t), over_c = excess(rest_max, log2e_t, rest_c);
   f.close = kBytes == 4 ? near_exponent(rest_c) : fabsf(rest_c) < 256.f;
   const float shift = kBytes == 4 ? 0.f : log2f(fabsf(coef));
   f.size = kBytes == 4 ? coef * exp2_approx(f.close ? -over_c : 0.f) : 1.f;
-  f.offset = kBytes == 4 ? -rest_c : shift - rest_c - over_c;
+  f.offset = kBytes == 4 ? -rest_c : __fsub_rn(__fsub_rn(shift, rest_c), over_c);
   f.sign = kBytes != 4 && coef < 0.f ? 0x80008000u : 0u;
   f.scaled = f.close ? log2e_t : 1.f; f.factor = f.close ? 1.f : log2e_t;
   f.minus = f.close ? f.offset : -rest_max; f.shift = f.close ? 0.f : shift;
