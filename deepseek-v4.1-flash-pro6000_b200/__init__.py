@@ -317,12 +317,15 @@ def constrain_logits(logits, history=None, history_len=None, repetition=1.0, pre
         raise ValueError("history_len without history")
     if (bias_ids is None) != (bias_values is None):
         raise ValueError("bias_ids and bias_values come together")
-    history_stride = biases = 0
+    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+    history_stride, history_ptr, biases = 0, None, 0
     if history is not None:
-        history_stride = _rows(_flat(history, torch.int32, "history", dev, history.numel()), (torch.int32,), "history", dev,
-                               (sequences, None))
+        _rows(_flat(history, torch.int32, "history", dev, history.numel()), (torch.int32,), "history", dev, (sequences, None))
+        history_stride, history_ptr = history.shape[1], history.data_ptr()
         if history_len is not None:
             _flat(history_len, torch.int32, "history_len", dev, sequences)
+            if history_stride == 0:    # (no columns, no address, and lengths are only looked at beside one: this one is never read from)
+                history_ptr = history_len.data_ptr()
     if penalties is not None:
         _flat(penalties, torch.float32, "penalties", dev, 3 * sequences)
     if draft_ids is not None:
@@ -337,9 +340,8 @@ def constrain_logits(logits, history=None, history_len=None, repetition=1.0, pre
         fill = lowest
     elif math.isfinite(fill):    # (within the type's range, and so within the argument's)
         fill = min(max(fill, lowest), -lowest)
-    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
     a = ConstrainArgs(C.sizeof(ConstrainArgs), sequences, rows_per_sequence, vocab, _ROW_TYPES[logits.dtype], biases, logits.data_ptr(),
-                      logits_stride, out.data_ptr(), out_stride, repetition, presence, frequency, fill, ptr(penalties), ptr(history), history_stride,
+                      logits_stride, out.data_ptr(), out_stride, repetition, presence, frequency, fill, ptr(penalties), history_ptr, history_stride,
                       ptr(history_len), ptr(draft_ids), ptr(bias_ids), ptr(bias_values), mask_ptr, mask_stride, status.data_ptr())
     _launch(dev, "ds41_b200_constrain_logits", lib().ds41_b200_constrain_logits, C.byref(a))
     return out, status
