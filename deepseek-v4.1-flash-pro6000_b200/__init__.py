@@ -557,8 +557,8 @@ def distill_loss(logits, teacher_ids, teacher_values, temperature=1.0, tail=Fals
 
 
 def distill_grad(logits, teacher_ids, teacher_values, stats, row_scale=None, temperature=1.0, tail=False, mask=None, out=None):
-    """The gradient of row_scale[r] * loss[r] by logits (the upstream gradient of each row's loss; None = 1; rows with 0 are not
-    read) from distill_loss's stats and the same other arguments.  out: None allocates; logits itself works in place.
+    """The gradient of row_scale[r] * loss[r] by logits (the upstream gradient of each row's loss; None = 1; rows with 0 are
+    padding, and get 0 whatever they hold) from distill_loss's stats and the same other arguments.  out: None allocates; logits itself works in place.
     Returns the gradient in the logits' type."""
     if stats.dim() != 2 or stats.shape[1] != 4:
         raise ValueError("stats must be [rows, 4]")
@@ -571,7 +571,7 @@ def distill_grad(logits, teacher_ids, teacher_values, stats, row_scale=None, tem
 
 def distill_loss_grad(logits, teacher_ids, teacher_values, row_scale=None, temperature=1.0, tail=False, mask=None, out=None):
     """Loss and gradient in one call that reads the logits once: distill_loss and distill_grad with row_scale known beforehand
-    (rows with 0 are not read: loss 0, gradient 0).  out: None allocates; logits itself works in place.
+    (rows with 0 are padding: loss 0, gradient 0, whatever they hold).  out: None allocates; logits itself works in place.
     Returns (loss fp32 [rows], gradient in the logits' type, status int32 [rows])."""
     rows, dev = logits.shape[0], logits.device
     loss = torch.empty(rows, dtype=torch.float32, device=dev)

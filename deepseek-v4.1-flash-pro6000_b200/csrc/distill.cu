@@ -13,7 +13,7 @@
 // next row's.  Two more warps: one gathers and reduces the next row's list and sets the last row's listed ids; the other brings the next
 // row's mask and, a row behind, takes the loss in FP64.  Three CTAs share an SM, each at another point of its row.  Small batches are bound
 // by the list's chain of loads and the exchange (8 rows of 129280 bf16 ids 8.1 us the loss, 10.5 with the gradient), masked ones by the
-// instructions of the mask (450 rows of 65537 fp32 ids 113 us, 0.38 of the copy rate).  Many long rows go through distill_stream.cuh.
+// instructions of the mask (450 rows of 65537 fp32 ids 114 us, 0.37 of the copy rate).  Many long rows go through distill_stream.cuh.
 #include "distill_stream.cuh"
 #include "row_team.cuh"
 #include "host_error.h"

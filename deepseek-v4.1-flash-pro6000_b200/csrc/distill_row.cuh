@@ -49,8 +49,8 @@ __device__ __forceinline__ float exp2_approx(float x) {   // 2 ulp; 0 for -inf a
 
 // The power of (x - m) c, with c = log2(e) / T, as that of x c - r with r = m c rounded: one fused multiply-add, its argument as exact, if
 // the rounding of r is made good for once a row.  That rounding is up to 2^-24 |r|, so the shortcut is for |r| below 2^24, where its power lies
-// between 0.7 and 1.42; at 2^31 it would be infinite or 0.  Beyond (logits of -1e8 and less in a row's masked places, a type's lowest values)
-// the power is that of (x - m) c.  (The rounding is asked for by name: what takes r must not get the product that it was rounded from.)
+// between 0.7 and 1.42; at 2^31 it would be infinite or 0.  Beyond (logits past 1.2e7 T: masked places, a type's lowest values) the power
+// is that of (x - m) c.  (The rounding is asked for by name: what takes r must not get the product that it was rounded from.)
 constexpr float kDisNear = 16777216.f;
 __device__ __forceinline__ bool near_exponent(float r) { return fabsf(r) < kDisNear; }
 __device__ __forceinline__ float rounded_product(float m, float c) { return __fmul_rn(m, c); }

@@ -3,8 +3,8 @@
 // its beginning, where the groups read last are still in the ring and those before them are the latest in the L2.  A group's copy
 // starts when the group in its place has been used, whichever pass or row it belongs to, so that copies are always on their way; the
 // list of a row, its reductions and the loss are one warp's work per row instead of one per slice.
-// The loss is bound by memory (1024 rows of 129280 fp32 ids 94 us, 0.86 of the copy rate); loss and gradient by two exponentials an id
-// (4096 bf16 rows 453 us, 0.72: its DRAM traffic at 0.86 of the copy rate, the exponential's pipe busy 0.53 of the time).  Two CTAs an SM: the rows of three
+// The loss is bound by memory (1024 rows of 129280 fp32 ids 95 us, 0.85 of the copy rate); loss and gradient by two exponentials an id
+// (4096 bf16 rows 456 us, 0.71: its DRAM traffic at 0.86 of the copy rate, the exponential's pipe busy 0.53 of the time).  Two CTAs an SM: the rows of three
 // do not fit the L2 until they are read again (511 us).
 #pragma once
 #include "distill_row.cuh"

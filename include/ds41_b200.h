@@ -412,7 +412,9 @@ int ds41_b200_constrain_logits(const ds41_b200_constrain_args *args, cudaStream_
  * The teacher's row is a list of ids and values, as ds41_b200_score_logits leaves them (top_ids, top_logprob) or as they were
  * stored; the student's is a row of logits.  No counterpart in the reference (it does not train).
  * With T = temperature, u_i = z_i / T over the ids that are allowed (mask bit set, z_i > -inf), q = softmax(u):
- *   entries: those whose id is in [0, vocab) and allowed count; entries of the same id add up; any other is padding
+ *   entries: those whose id is in [0, vocab) and allowed count; entries of the same id add up.  An id outside [0, vocab) is padding and
+ *            its value means nothing.  An entry in the vocabulary that is not allowed has no share of p, but its value is one of the
+ *            list's: it is checked, and with tail = 1 counts in the list's sum
  *   tail = 0: p_j = exp(value_j / T) over the list, normalised to 1
  *   tail = 1 (T = 1): p_j = exp(value_j), values being log-probabilities over the teacher's whole row; the ids outside the list have
  *             together rest = max(0, 1 - sum of the list) (nothing where every allowed id is listed); all normalised to 1
@@ -423,7 +425,7 @@ int ds41_b200_constrain_logits(const ds41_b200_constrain_args *args, cudaStream_
  * rounded once to the rows' type.
  * stats [rows, 4]: the largest allowed logit, ln sum exp((z - largest) / T), and the same two over the allowed ids outside the list
  * (-inf where there are none): what _grad needs of _loss.  row_scale [rows] (NULL = 1): the gradient of the caller's loss by each row's;
- * a row whose scale is 0 (padding) is not read: gradient 0, loss, stats and status 0.
+ * a row whose scale is 0 is padding: whatever its logits, list, mask and stats hold, its gradient, loss, stats and status are 0.
  * status[r]: 0, or the first that holds of
  *   DS41_B200_ROW_NONFINITE (the value of an entry in the vocabulary is NaN or +inf, or an allowed logit that an entry names is),
  *   DS41_B200_ROW_NOT_NORMALIZED (tail: the list's probabilities add up to more than 1.01),
